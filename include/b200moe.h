@@ -167,6 +167,28 @@ int b200moe_gemm_bf16_nvfp4(const void* a, int64_t a_stride, const void* b_q, co
                             int64_t m, int64_t n, int64_t k, int64_t out_stride, void* workspace, int64_t workspace_bytes,
                             int32_t* status, void* stream);
 
+/* ---- Linear layers in 8 bits: rows as codes (int8 or E4M3) with one fp32 scale per row, value = code * scale. The reference operator has
+ * no counterpart to these or to the token sorting below. */
+#define B200MOE_BF16 0 /* types of rows */
+#define B200MOE_FP16 1
+#define B200MOE_FP32 2
+#define B200MOE_INT8 0 /* types of codes: -127..127, or E4M3 up to 448 */
+#define B200MOE_E4M3 1
+
+/* RMS norm with the residual's addition and a quantised output, for each of `rows` rows of 1..32768 columns:
+ *   h = x + residual,  y = h * (mean(h^2) + eps)^-1/2 * weight,  scale = max|y| / Q,  q = round(y / scale)   (Q = 127 or 448).
+ * residual may be NULL (h = x); hidden (h) and normed (y), in the rows' type `dtype`, are written where not NULL. hidden may be x or
+ * residual itself. weight: [cols] in the rows' type or fp32. Strides in elements between rows (0 repeats one input row). Sums in fp32; h is not
+ * rounded before the norm. A row whose max|y| is below 2^-116 has scale 0 and codes 0; a row with a NaN or an infinity in it, or
+ * with a sum of squares beyond fp32, has scale NaN and codes 0. Any width and alignment; 16-byte aligned rows are the fast ones. */
+int b200moe_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                             int32_t weight_dtype, int64_t rows, int64_t cols, float eps, int32_t dtype, int32_t q_type, void* q,
+                             int64_t q_stride, float* scale, void* hidden, int64_t hidden_stride, void* normed, int64_t normed_stride,
+                             void* stream);
+/* SwiGLU with a quantised output: x = [gate | up] of 2 * cols columns, y = gate * sigmoid(gate) * up, scale and q as above. */
+int b200moe_swiglu_quantize(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int32_t dtype, int32_t q_type, void* q,
+                            int64_t q_stride, float* scale, void* stream);
+
 /* Layer life cycle. Replaces moe_init / moe_run of NV/candidate/nvfp4_moe.cu:6618, :9496 (bound there through
  * ctypes, NV/candidate/solution.py:96-102). create allocates the workspace on the current device. */
 int b200moe_create(const b200moe_config* cfg, b200moe_handle* out);

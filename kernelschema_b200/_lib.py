@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(HERE, "libb200moe.so")
 
 ABI_VERSION = 3
 SF_ROW_MAJOR, SF_TILED = 0, 1
+BF16, FP16, FP32 = 0, 1, 2
+INT8, E4M3 = 0, 1
 
 
 class Config(C.Structure):
@@ -97,6 +99,11 @@ SIGNATURES = {
                                   C.c_void_p]),
     "b200moe_route_map_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
                                   + [C.c_void_p] * 9 + [C.c_int64, C.c_void_p]),
+    "b200moe_rmsnorm_quantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_float,
+                                           C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                           C.c_void_p]),
+    "b200moe_swiglu_quantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                          C.c_void_p]),
     "b200moe_ep_shared_alloc": (C.c_int, [C.c_int64, C.POINTER(C.c_void_p), C.c_void_p]),
     "b200moe_ep_shared_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "b200moe_ep_shared_close": (C.c_int, [C.c_void_p]),

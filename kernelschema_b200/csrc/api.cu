@@ -668,6 +668,40 @@ int b200moe_combine(const void* rows, const int32_t* row_of, const float* weight
   return cuda_fail(launch_finalize(rows, row_of, weight_of_row, T, slots, hidden, out, out_stride, (cudaStream_t)stream), "combine");
 }
 
+int b200moe_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int32_t weight_dtype,
+                             int64_t rows, int64_t cols, float eps, int32_t dtype, int32_t q_type, void* q, int64_t q_stride, float* scale,
+                             void* hidden, int64_t hidden_stride, void* normed, int64_t normed_stride, void* stream) {
+  if (rows < 0 || rows > INT32_MAX || cols <= 0 || cols > kRowQuantMaxCols)
+    return fail(775, "rmsnorm_quantize: need 0 <= rows < 2^31 and 0 < cols <= %d, got %lld x %lld", kRowQuantMaxCols, (long long)rows, (long long)cols);
+  if (dtype < kBf16 || dtype > kF32 || q_type < kInt8 || q_type > kE4m3 || (weight_dtype != dtype && weight_dtype != kF32))
+    return fail(776, "rmsnorm_quantize: unknown dtype or q_type, or a weight that is neither of the rows' type nor fp32");
+  if (!(eps >= 0.f)) return fail(776, "rmsnorm_quantize: eps must not be negative");
+  if (!rows) return 0;
+  if (!x || !weight || !q || !scale) return fail(777, "rmsnorm_quantize: null pointer");
+  if (x_stride < 0 || residual_stride < 0 || q_stride < cols || (hidden && hidden_stride < cols) || (normed && normed_stride < cols))
+    return fail(778, "rmsnorm_quantize: a stride between output rows is below cols, or an input's is negative");
+  const uintptr_t size = dtype == kF32 ? 4 : 2;
+  if ((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)hidden | (uintptr_t)normed) & (size - 1)) || ((uintptr_t)weight & (weight_dtype == kF32 ? 3 : 1)) ||
+      ((uintptr_t)scale & 3))
+    return fail(778, "rmsnorm_quantize: a tensor is not aligned to its elements");
+  RmsNormParams p{x, residual, weight, (uint8_t*)q, scale, hidden, normed, rows, x_stride, residual_stride, q_stride, hidden_stride, normed_stride,
+                  (int)cols, dtype, weight_dtype == kF32 && dtype != kF32, q_type, eps};
+  return cuda_fail(launch_rmsnorm_quantize(p, (cudaStream_t)stream), "rmsnorm_quantize");
+}
+
+int b200moe_swiglu_quantize(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int32_t dtype, int32_t q_type, void* q, int64_t q_stride,
+                            float* scale, void* stream) {
+  if (rows < 0 || rows > INT32_MAX || cols <= 0 || cols > kRowQuantMaxCols)
+    return fail(779, "swiglu_quantize: need 0 <= rows < 2^31 and 0 < cols <= %d, got %lld x %lld", kRowQuantMaxCols, (long long)rows, (long long)cols);
+  if (dtype < kBf16 || dtype > kF32 || q_type < kInt8 || q_type > kE4m3) return fail(776, "swiglu_quantize: unknown dtype or q_type");
+  if (!rows) return 0;
+  if (!x || !q || !scale) return fail(777, "swiglu_quantize: null pointer");
+  if (x_stride < 0 || q_stride < cols) return fail(778, "swiglu_quantize: q_stride must be >= cols and x_stride not negative");
+  if (((uintptr_t)x & (dtype == kF32 ? 3 : 1)) || ((uintptr_t)scale & 3)) return fail(778, "swiglu_quantize: a tensor is not aligned to its elements");
+  SwigluParams p{x, (uint8_t*)q, scale, rows, x_stride, q_stride, (int)cols, dtype, q_type};
+  return cuda_fail(launch_swiglu_quantize(p, (cudaStream_t)stream), "swiglu_quantize");
+}
+
 int b200moe_route_map_noalloc(const int32_t* ids, const float* weights, int32_t T, int32_t top_k, int32_t num_shared,
                               int32_t num_experts, int32_t offset, int32_t* counts, int32_t* seg_start, int32_t* tile_expert,
                               int32_t* tile_row0, int32_t* tile_rows, int32_t* totals, int32_t* row_of, int32_t* tok_of_row,

@@ -206,6 +206,29 @@ int launch_gemm_w4a16_expand(const void* a, int64_t a_stride, const void* b_q, c
 int64_t gemm_w4a16_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int make_sf_map(CUtensorMap* map, const void* base, uint64_t n_chunks);
 
+// ---- rows in 8 bits with one scale each (rowquant.cu)
+enum { kBf16 = 0, kF16 = 1, kF32 = 2 };      // types of rows: B200MOE_BF16, ...
+enum { kInt8 = 0, kE4m3 = 1 };               // types of codes: B200MOE_INT8, ...
+constexpr int kRowQuantMaxCols = 32768;      // a row stays in one block's registers
+struct RmsNormParams {
+  const void *x, *residual, *weight;         // residual may be null
+  uint8_t* q;
+  float* scale;
+  void *hidden, *normed;                     // x + residual and the normed row in the rows' type; each may be null
+  int64_t rows, x_stride, residual_stride, q_stride, hidden_stride, normed_stride;   // strides in elements
+  int cols, dtype, weight_f32, q_type;
+  float eps;
+};
+struct SwigluParams {
+  const void* x;                             // [rows, 2 * cols]: gate, up
+  uint8_t* q;
+  float* scale;
+  int64_t rows, x_stride, q_stride;
+  int cols, dtype, q_type;
+};
+int launch_rmsnorm_quantize(const RmsNormParams& p, cudaStream_t st);
+int launch_swiglu_quantize(const SwigluParams& p, cudaStream_t st);
+
 // ---- expert-parallel exchange over peer memory (ep_exchange.cu)
 constexpr int kEpMaxRanks = 16;
 // int32 fields of a rank's control block, each kEpMaxRanks wide and indexed by the peer that writes it

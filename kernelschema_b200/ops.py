@@ -224,6 +224,92 @@ def mm_bf16_nvfp4(a: torch.Tensor, b: torch.Tensor, b_descale: torch.Tensor, alp
     return out
 
 
+_ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
+_CODE_TYPES = {torch.int8: _lib.INT8, torch.float8_e4m3fn: _lib.E4M3}
+
+
+def _here(*tensors) -> None:
+    """The tensors of a call are on the current device, whose current stream it uses."""
+    for t in tensors:
+        if t is not None:
+            at = t.get_device()
+            if at < 0:
+                raise ValueError("libb200moe operates on CUDA tensors only")
+            if at != torch._C._cuda_getDevice():
+                raise ValueError(f"a tensor is on cuda:{at}, the current device is cuda:{torch._C._cuda_getDevice()}: call under torch.cuda.device({at})")
+
+
+def _unit_rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """Elements between rows; a single row has no next one, whatever its stride says."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _out_rows(out, shape, dtype, name: str, device) -> torch.Tensor:
+    """A caller's buffer for rows of `shape`, checked, or a new one."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or (out.dim() == 2 and (out.shape[1] > 1 and out.stride(1) != 1 or _row_stride(out) < shape[1])) \
+            or (out.dim() == 1 and not out.is_contiguous()):
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} with unit inner stride and rows that do not overlap")
+    return out
+
+
+def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                     dtype: torch.dtype = torch.int8, normed: bool = False, out=None):
+    """Residual addition, RMS norm and 8-bit quantisation of rows in one pass -> (q, scale, hidden, normed).
+
+    h = x + residual, y = h * (mean(h^2) + eps)^-1/2 * weight, scale = max|y| / Q (fp32, one per row), q = round(y / scale): int8 (Q = 127)
+    or float8_e4m3fn (Q = 448), what `mm_8bit` takes. x, residual: bf16, fp16 or fp32 [T, H], H <= 32768; weight [H] in the same type or
+    fp32. ``hidden`` is h in x's type (x itself without a residual); ``normed`` is y in x's type where asked for, else None. ``out`` = (q,
+    scale, hidden, normed): caller-owned buffers, each may be None; hidden may be x or residual themselves (in place).
+    h and the sums are fp32, and h is not rounded before the norm. A row of zeros (max|y| < 2^-116) has scale 0; a row with a NaN or an infinity, or whose
+    squares' sum leaves fp32, has scale NaN and codes 0."""
+    if x.dim() != 2 or x.dtype not in _ROW_TYPES or (residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape)):
+        raise ValueError("rmsnorm_quantize expects bf16, fp16 or fp32 [T, H] and a residual like it")
+    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight must be [{x.shape[1]}] in x's type or float32")
+    if dtype not in _CODE_TYPES:
+        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
+    q, scale, hidden, norm = out if out is not None else (None, None, None, None)
+    _here(x, weight, residual, q, scale, hidden, norm)
+    x, weight = _unit_rows(x), weight.contiguous()
+    residual = None if residual is None else _unit_rows(residual)
+    t, h = x.shape
+    q = _out_rows(q, (t, h), dtype, "q", x.device)
+    scale = _out_rows(scale, (t,), torch.float32, "scale", x.device)
+    if residual is not None or hidden is not None:
+        hidden = _out_rows(hidden, (t, h), x.dtype, "hidden", x.device)
+    if normed or norm is not None:
+        norm = _out_rows(norm, (t, h), x.dtype, "normed", x.device)
+    _lib.check(_lib.load().b200moe_rmsnorm_quantize(
+        x.data_ptr(), _row_stride(x), _ptr(residual), 0 if residual is None else _row_stride(residual), weight.data_ptr(), _ROW_TYPES[weight.dtype], t, h,
+        eps, _ROW_TYPES[x.dtype], _CODE_TYPES[dtype], q.data_ptr(), _row_stride(q), scale.data_ptr(), _ptr(hidden), 0 if hidden is None else _row_stride(hidden),
+        _ptr(norm), 0 if norm is None else _row_stride(norm), _stream()), "b200moe_rmsnorm_quantize")
+    return q, scale, x if hidden is None else hidden, norm
+
+
+def swiglu_quantize(x: torch.Tensor, dtype: torch.dtype = torch.int8, out=None):
+    """x = [gate | up] (bf16, fp16 or fp32 [T, 2I], I <= 32768) -> (q [T, I], scale fp32 [T]) of gate * sigmoid(gate) * up: the step between the two 8-bit
+    products of a feed-forward layer or an expert. dtype, scales, special rows and ``out`` = (q, scale) as in `rmsnorm_quantize`."""
+    if x.dim() != 2 or x.dtype not in _ROW_TYPES or x.shape[1] % 2 or not x.shape[1]:
+        raise ValueError("swiglu_quantize expects bf16, fp16 or fp32 [T, 2I]")
+    if dtype not in _CODE_TYPES:
+        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
+    q, scale = out if out is not None else (None, None)
+    _here(x, q, scale)
+    x = _unit_rows(x)
+    t, i = x.shape[0], x.shape[1] // 2
+    q = _out_rows(q, (t, i), dtype, "q", x.device)
+    scale = _out_rows(scale, (t,), torch.float32, "scale", x.device)
+    _lib.check(_lib.load().b200moe_swiglu_quantize(x.data_ptr(), _row_stride(x), t, i, _ROW_TYPES[x.dtype], _CODE_TYPES[dtype], q.data_ptr(),
+                                                   _row_stride(q), scale.data_ptr(), _stream()), "b200moe_swiglu_quantize")
+    return q, scale
+
+
 def combine(rows: torch.Tensor, row_of: torch.Tensor, weight_of_row: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """out[t] = bf16(sum_s rows[row_of[t, s]] * weight_of_row[row_of[t, s]]) (reference.py:91-92), slots ascending."""
     _need_cuda(rows, row_of, weight_of_row, out)
