@@ -189,6 +189,18 @@ int b200moe_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residu
 int b200moe_swiglu_quantize(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int32_t dtype, int32_t q_type, void* q,
                             int64_t q_stride, float* scale, void* stream);
 
+/* GEMM of 8-bit rows: out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k]. a [M, K] and b [N, K] both int8 (sums exact in int32) or both
+ * E4M3 (sums in fp32), K % 16 == 0 and K <= 131071, 16-byte aligned, a_stride (bytes between rows of a) a multiple of 16; scales fp32; out
+ * [M, N] bf16, fp16 or fp32, any N and out_stride. status as in b200moe_gemm_nvfp4. */
+int b200moe_gemm_8bit(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, void* out, int64_t m,
+                      int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type, int32_t* status, void* stream);
+/* The same over segments of rows, each with its own weights: rows offsets[e] .. offsets[e + 1] - 1 (device int32 [experts + 1], ascending) times
+ * b[e] of b [experts, N, K] with b_scale [experts, N]. Segments may be empty. Rows of no segment are left as they are, or become zero
+ * with zero_rest. Offsets are cut to 0..M and to ascending order, so no value of theirs reaches memory outside the tensors. experts <= 1024. */
+int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale,
+                              const int32_t* offsets, int32_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride,
+                              int32_t code, int32_t out_type, int32_t zero_rest, int32_t* status, void* stream);
+
 /* Layer life cycle. Replaces moe_init / moe_run of NV/candidate/nvfp4_moe.cu:6618, :9496 (bound there through
  * ctypes, NV/candidate/solution.py:96-102). create allocates the workspace on the current device. */
 int b200moe_create(const b200moe_config* cfg, b200moe_handle* out);

@@ -702,6 +702,37 @@ int b200moe_swiglu_quantize(const void* x, int64_t x_stride, int64_t rows, int64
   return cuda_fail(launch_swiglu_quantize(p, (cudaStream_t)stream), "swiglu_quantize");
 }
 
+static int gemm_8bit_checked(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
+                             int64_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type, int zero_rest,
+                             int32_t* status, void* stream) {
+  if (m < 0 || n <= 0 || k <= 0 || k % 16 || k > kGemm8MaxK)
+    return fail(784, "gemm_8bit: M=%lld N=%lld K=%lld need K %% 16 == 0 and K <= %lld", (long long)m, (long long)n, (long long)k, (long long)kGemm8MaxK);
+  if (m > (1 << 30) || n > (1 << 30) || n * (experts ? experts : 1) > (1ll << 30)) return fail(784, "gemm_8bit: more than 2^30 rows are not supported");
+  if (code < kInt8 || code > kE4m3 || out_type < kBf16 || out_type > kF32) return fail(785, "gemm_8bit: unknown type of codes or output");
+  if (!m) return 0;
+  if (!a || !a_scale || !b || !b_scale || !out) return fail(786, "gemm_8bit: null pointer");
+  if (((uintptr_t)a | (uintptr_t)b) & 15) return fail(783, "gemm_8bit: operands must be 16-byte aligned");
+  if (a_stride < k || a_stride % 16) return fail(783, "gemm_8bit: a_stride must be >= K and a multiple of 16");
+  const uintptr_t size = out_type == kF32 ? 4 : 2;
+  if (out_stride < n || ((uintptr_t)out & (size - 1)) || (((uintptr_t)a_scale | (uintptr_t)b_scale | (uintptr_t)offsets | (uintptr_t)status) & 3))
+    return fail(783, "gemm_8bit: out_stride must be >= N, and every tensor aligned to its elements");
+  Gemm8Params p{a_scale, b_scale, offsets, out, out_stride, status, (int)m, (int)n, (int)k, (int)experts, code, out_type, zero_rest};
+  return cuda_fail(launch_gemm_8bit(a, a_stride, b, p, (cudaStream_t)stream), "gemm_8bit");
+}
+
+int b200moe_gemm_8bit(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, void* out, int64_t m, int64_t n,
+                      int64_t k, int64_t out_stride, int32_t code, int32_t out_type, int32_t* status, void* stream) {
+  return gemm_8bit_checked(a, a_stride, a_scale, b, b_scale, nullptr, 0, out, m, n, k, out_stride, code, out_type, 0, status, stream);
+}
+
+int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
+                              int32_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type,
+                              int32_t zero_rest, int32_t* status, void* stream) {
+  if (experts <= 0 || experts > kGemm8MaxExperts) return fail(784, "gemm_8bit_grouped: need 0 < experts <= %d", kGemm8MaxExperts);
+  if (m > 0 && !offsets) return fail(786, "gemm_8bit_grouped: offsets is null");
+  return gemm_8bit_checked(a, a_stride, a_scale, b, b_scale, offsets, experts, out, m, n, k, out_stride, code, out_type, zero_rest != 0, status, stream);
+}
+
 int b200moe_route_map_noalloc(const int32_t* ids, const float* weights, int32_t T, int32_t top_k, int32_t num_shared,
                               int32_t num_experts, int32_t offset, int32_t* counts, int32_t* seg_start, int32_t* tile_expert,
                               int32_t* tile_row0, int32_t* tile_rows, int32_t* totals, int32_t* row_of, int32_t* tok_of_row,

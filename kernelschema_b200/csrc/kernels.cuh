@@ -229,6 +229,21 @@ struct SwigluParams {
 int launch_rmsnorm_quantize(const RmsNormParams& p, cudaStream_t st);
 int launch_swiglu_quantize(const SwigluParams& p, cudaStream_t st);
 
+// ---- GEMM of 8-bit rows (gemm_8bit.cu)
+constexpr int kGemm8MaxExperts = 1024;
+constexpr int64_t kGemm8MaxK = 131071;       // 128 * 128 * K stays below 2^31: an int32 sum of int8 products is exact
+struct Gemm8Params {
+  const float *a_scale, *b_scale;            // [M]; [N] or [experts, N]
+  const int32_t* offsets;                    // grouped: [experts + 1] first rows of the segments
+  void* out;
+  int64_t out_stride;
+  int32_t* status;
+  int M, N, K, experts;                      // experts 0: dense
+  int code, out_type;                        // kInt8 / kE4m3; kBf16 / kF16 / kF32
+  int zero_rest;                             // grouped: rows of no segment become zero
+};
+int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
+
 // ---- expert-parallel exchange over peer memory (ep_exchange.cu)
 constexpr int kEpMaxRanks = 16;
 // int32 fields of a rank's control block, each kEpMaxRanks wide and indexed by the peer that writes it

@@ -310,6 +310,61 @@ def swiglu_quantize(x: torch.Tensor, dtype: torch.dtype = torch.int8, out=None):
     return q, scale
 
 
+def _mm_8bit_args(a, a_scale, b, b_scale, lead, out, out_dtype, status, offsets=None):
+    """Checks that `mm_8bit` (lead = ()) and `mm_8bit_grouped` (lead = (experts,)) share -> (a, a_scale, b, b_scale, out)."""
+    if a.dim() != 2 or b.dim() != 2 + len(lead) or a.dtype not in _CODE_TYPES or b.dtype != a.dtype:
+        raise ValueError("a [M, K] and b [N, K] (experts: [E, N, K]) must both be int8 or both float8_e4m3fn")
+    m, k = a.shape
+    n = b.shape[-2]
+    if b.shape[-1] != k or k % 16 or not k or not n:
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} must share K, a multiple of 16")
+    if a_scale.dtype != torch.float32 or a_scale.numel() != m or b_scale.dtype != torch.float32 or b_scale.numel() != b.numel() // k:
+        raise ValueError("a_scale must hold one fp32 value per row of a, b_scale one per row of b")
+    if out_dtype not in _ROW_TYPES:
+        raise ValueError("out_dtype must be bfloat16, float16 or float32")
+    if status is not None and (status.dtype != torch.int32 or not status.numel()):
+        raise ValueError("status must be an int32 tensor")
+    _here(a, a_scale, b, b_scale, out, status, offsets)
+    a = _unit_rows(a)
+    if _row_stride(a) % 16 or a.data_ptr() % 16:
+        a = a.contiguous() if not a.is_contiguous() else a.clone()
+    if not b.is_contiguous() or b.data_ptr() % 16:
+        raise ValueError("b must be contiguous and 16-byte aligned")
+    return a, a_scale.contiguous(), b, b_scale.contiguous(), _out_rows(out, (m, n), out_dtype, "out", a.device)
+
+
+def mm_8bit(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: torch.Tensor | None = None,
+            out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
+    """out[M, N] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k]: activations in 8 bits with one fp32 scale per token (as `rmsnorm_quantize` and
+    `swiglu_quantize` leave them) times weights [N, K] in 8 bits with one per output channel, both int8 (sums exact in int32) or both
+    float8_e4m3fn (sums in fp32). K % 16 == 0, K <= 131071; any M and N. out: bf16, fp16 or fp32 (``out_dtype``, which a given ``out`` must have)."""
+    if out is not None:
+        out_dtype = out.dtype
+    a, a_scale, b, b_scale, out = _mm_8bit_args(a, a_scale, b, b_scale, (), out, out_dtype, status)
+    _lib.check(_lib.load().b200moe_gemm_8bit(a.data_ptr(), _row_stride(a), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), out.data_ptr(),
+                                             a.shape[0], b.shape[0], a.shape[1], _row_stride(out), _CODE_TYPES[a.dtype], _ROW_TYPES[out_dtype],
+                                             _ptr(status), _stream()), "b200moe_gemm_8bit")
+    return out
+
+
+def mm_8bit_grouped(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, offsets: torch.Tensor,
+                    out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
+    """`mm_8bit` over the experts' segments of sorted rows: rows offsets[e] .. offsets[e + 1] - 1 times b[e]. offsets int32 [E + 1] on the device
+    (`route_sort` makes it); b [E, N, K], b_scale [E, N], E <= 1024. Rows of no segment are zero in a new output and left as they are in a given one."""
+    if out is not None:
+        out_dtype = out.dtype
+    if b.dim() != 3 or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != b.shape[0] + 1:
+        raise ValueError("b must be [E, N, K] and offsets int32 [E + 1]")
+    fresh = out is None
+    a, a_scale, b, b_scale, out = _mm_8bit_args(a, a_scale, b, b_scale, (b.shape[0],), out, out_dtype, status, offsets)
+    offsets = offsets.contiguous()
+    _lib.check(_lib.load().b200moe_gemm_8bit_grouped(a.data_ptr(), _row_stride(a), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
+                                                     offsets.data_ptr(), b.shape[0], out.data_ptr(), a.shape[0], b.shape[1], a.shape[1],
+                                                     _row_stride(out), _CODE_TYPES[a.dtype], _ROW_TYPES[out_dtype], int(fresh), _ptr(status),
+                                                     _stream()), "b200moe_gemm_8bit_grouped")
+    return out
+
+
 def combine(rows: torch.Tensor, row_of: torch.Tensor, weight_of_row: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """out[t] = bf16(sum_s rows[row_of[t, s]] * weight_of_row[row_of[t, s]]) (reference.py:91-92), slots ascending."""
     _need_cuda(rows, row_of, weight_of_row, out)

@@ -49,3 +49,36 @@ def test_rowquant_abi_refusals(lib):
     assert swi(cols=0) == 779 and swi(cols=32769) == 779 and swi(dt=-1) == 776 and swi(qt=5) == 776 and swi(x=None) == 777
     assert swi(x=18, dt=2) == 778 and swi(qs=1) == 778 and swi(xs=-1) == 778 and swi(rows=0, q=None) == 0
     assert b"swiglu_quantize" in lib.b200moe_last_error()
+
+
+def test_gemm_8bit_refusals(lib):
+    i8 = torch.int8
+    f = torch.float32
+    ok = dict(a=z(4, 64, dtype=i8), sa=z(4, dtype=f), b=z(32, 64, dtype=i8), sb=z(32, dtype=f))
+
+    def mm(out=None, out_dtype=torch.bfloat16, status=None, **over):
+        v = dict(ok, **over)
+        return ks.mm_8bit(v["a"], v["sa"], v["b"], v["sb"], out, out_dtype, status)
+
+    for over in (dict(),                                                                              # not on a device
+                 dict(a=z(4, 64)), dict(b=z(32, 64, dtype=torch.float8_e4m3fn)), dict(b=z(32, 48, dtype=i8)), dict(a=z(4, 60, dtype=i8), b=z(32, 60, dtype=i8)),
+                 dict(sa=z(5, dtype=f)), dict(sb=z(31, dtype=f)), dict(sa=z(4)), dict(out_dtype=torch.int32), dict(a=z(2, 4, 64, dtype=i8)),
+                 dict(status=z(1, dtype=f)), dict(a=z(4, 0, dtype=i8), b=z(32, 0, dtype=i8)), dict(b=z(0, 64, dtype=i8), sb=z(0, dtype=f))):
+        with pytest.raises(ValueError):
+            mm(**over)
+    b3, s3, off = z(3, 32, 64, dtype=i8), z(3, 32, dtype=f), z(4, dtype=torch.int32)
+    for args in ((ok["a"], ok["sa"], b3, s3, off), (ok["a"], ok["sa"], b3, s3, z(3, dtype=torch.int32)), (ok["a"], ok["sa"], b3, s3, z(4, dtype=torch.int64)),
+                 (ok["a"], ok["sa"], ok["b"], ok["sb"], off), (ok["a"], ok["sa"], b3, ok["sb"], off)):
+        with pytest.raises(ValueError):
+            ks.mm_8bit_grouped(*args)
+
+    def abi(a=16, a_st=64, sa=16, b=16, sb=16, out=16, m=4, n=32, k=64, o_st=32, code=0, ot=0, off=None, e=None):
+        if e is None:
+            return lib.b200moe_gemm_8bit(a, a_st, sa, b, sb, out, m, n, k, o_st, code, ot, None, None)
+        return lib.b200moe_gemm_8bit_grouped(a, a_st, sa, b, sb, off, e, out, m, n, k, o_st, code, ot, 0, None, None)
+
+    assert abi(k=60) == 784 and abi(k=131072) == 784 and abi(n=0) == 784 and abi(m=-1) == 784 and abi(m=(1 << 30) + 1) == 784
+    assert abi(code=2) == 785 and abi(ot=3) == 785 and abi(a=None) == 786 and abi(sb=None) == 786 and abi(out=None) == 786
+    assert abi(a=24) == 783 and abi(b=8) == 783 and abi(a_st=48) == 783 and abi(a_st=72) == 783 and abi(o_st=31) == 783 and abi(out=17) == 783
+    assert abi(m=0, a=None) == 0 and abi(e=0, off=16) == 784 and abi(e=1025, off=16) == 784 and abi(e=3) == 786 and abi(e=3, off=18) == 783
+    assert abi(e=1024, off=16, n=1 << 21) == 784
