@@ -201,6 +201,29 @@ int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_sc
                               const int32_t* offsets, int32_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride,
                               int32_t code, int32_t out_type, int32_t zero_rest, int32_t* status, void* stream);
 
+/* ---- Tokens in the order of their experts, and back, with the gradients (training and serving; no layer handle, no padding rows).
+ * route_sort: stable counting sort of the T * top_k routes by expert id. ids [T, top_k] (ids_stride elements between tokens; ids outside
+ * [0, num_experts) are no route, the same id twice in a token is two). offsets [num_experts + 1]: first row of each expert's segment, the last = routes
+ * that have an expert; row_of [T * top_k]: row of a route or -1; route_of_row [T * top_k]: t * top_k + k of a row, -1 behind the last segment.
+ * workspace: device memory of b200moe_route_sort_workspace_bytes (0 for small builds, -1 for sizes that are refused), overwritten by each call.
+ * num_experts <= 1024, fewer than 2^31 routes. */
+int64_t b200moe_route_sort_workspace_bytes(int64_t num_tokens, int32_t top_k, int32_t num_experts);
+int b200moe_route_sort(const int32_t* ids, int64_t ids_stride, int64_t num_tokens, int32_t top_k, int32_t num_experts, int32_t* offsets,
+                       int32_t* row_of, int32_t* route_of_row, void* workspace, int64_t workspace_bytes, void* stream);
+/* rows[row_of[t, k]] = x[t], rows of any type as row_bytes bytes (x_stride bytes between tokens); rows [T * top_k] contiguous, zero from
+ * *valid_rows (device: the last of the offsets) on. Its gradient is b200moe_unsort_rows without weights. */
+int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64_t row_bytes, const int32_t* row_of, int32_t top_k,
+                      const int32_t* valid_rows, void* rows, void* stream);
+/* out[t] = sum_k weights[t, k] * rows[row_of[t, k]] (weights NULL: 1), slots in ascending k, fp32, rounded once; row_of outside 0..num_rows - 1 is
+ * skipped, a token without routes becomes 0. */
+int b200moe_unsort_rows(const void* rows, int64_t rows_stride, int64_t num_rows, const int32_t* row_of, const float* weights, int64_t num_tokens,
+                        int32_t top_k, int64_t cols, int32_t dtype, void* out, int64_t out_stride, void* stream);
+/* Gradients of the above: grad_rows[row_of[t, k]] = weights[t, k] * grad_out[t] ([T * top_k, cols] contiguous, zero from *valid_rows on),
+ * grad_weights[t, k] = <rows[row_of[t, k]], grad_out[t]> (fp32; 0 where there is no route). Either may be NULL. */
+int b200moe_unsort_rows_backward(const void* grad_out, int64_t grad_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
+                                 const float* weights, int64_t num_tokens, int32_t top_k, int64_t cols, int32_t dtype,
+                                 const int32_t* valid_rows, void* grad_rows, float* grad_weights, void* stream);
+
 /* Layer life cycle. Replaces moe_init / moe_run of NV/candidate/nvfp4_moe.cu:6618, :9496 (bound there through
  * ctypes, NV/candidate/solution.py:96-102). create allocates the workspace on the current device. */
 int b200moe_create(const b200moe_config* cfg, b200moe_handle* out);

@@ -108,6 +108,14 @@ SIGNATURES = {
                                     C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
     "b200moe_gemm_8bit_grouped": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64,
                                             C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "b200moe_route_sort_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32]),
+    "b200moe_route_sort": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_int64, C.c_void_p]),
+    "b200moe_sort_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200moe_unsort_rows": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_void_p,
+                                      C.c_int64, C.c_void_p]),
+    "b200moe_unsort_rows_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
+                                               C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200moe_ep_shared_alloc": (C.c_int, [C.c_int64, C.POINTER(C.c_void_p), C.c_void_p]),
     "b200moe_ep_shared_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "b200moe_ep_shared_close": (C.c_int, [C.c_void_p]),

@@ -733,6 +733,72 @@ int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_sc
   return gemm_8bit_checked(a, a_stride, a_scale, b, b_scale, offsets, experts, out, m, n, k, out_stride, code, out_type, zero_rest != 0, status, stream);
 }
 
+static int order_sizes(const char* what, int64_t T, int32_t top_k) {
+  if (T < 0 || top_k <= 0 || T * top_k > INT32_MAX || T > INT32_MAX) return fail(787, "%s: need tokens >= 0, top_k > 0 and fewer than 2^31 routes", what);
+  return 0;
+}
+
+int64_t b200moe_route_sort_workspace_bytes(int64_t num_tokens, int32_t top_k, int32_t num_experts) {
+  if (order_sizes("route_sort", num_tokens, top_k) || num_experts <= 0 || num_experts > kOrderMaxExperts) return -1;
+  return route_sort_workspace_bytes(num_tokens * top_k, num_experts);
+}
+
+int b200moe_route_sort(const int32_t* ids, int64_t ids_stride, int64_t num_tokens, int32_t top_k, int32_t num_experts, int32_t* offsets, int32_t* row_of,
+                       int32_t* route_of_row, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = order_sizes("route_sort", num_tokens, top_k)) return rc;
+  if (num_experts <= 0 || num_experts > kOrderMaxExperts) return fail(787, "route_sort: num_experts must be in 1..%d", kOrderMaxExperts);
+  if (!offsets || (num_tokens && (!ids || !row_of || !route_of_row))) return fail(788, "route_sort: null pointer");
+  if (ids_stride < 0) return fail(789, "route_sort: ids_stride must not be negative");
+  if (((uintptr_t)ids | (uintptr_t)offsets | (uintptr_t)row_of | (uintptr_t)route_of_row | (uintptr_t)workspace) & 3)
+    return fail(789, "route_sort: tensors must be 4-byte aligned");
+  const int64_t need = route_sort_workspace_bytes(num_tokens * top_k, num_experts);
+  if (need && (!workspace || workspace_bytes < need)) return fail(771, "route_sort: needs %lld bytes of workspace", (long long)need);
+  return cuda_fail(launch_route_sort(ids, ids_stride, num_tokens, top_k, num_experts, offsets, row_of, route_of_row, workspace, (cudaStream_t)stream),
+                   "route_sort");
+}
+
+int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64_t row_bytes, const int32_t* row_of, int32_t top_k,
+                      const int32_t* valid_rows, void* rows, void* stream) {
+  if (int rc = order_sizes("sort_rows", num_tokens, top_k)) return rc;
+  if (row_bytes <= 0 || row_bytes > (1 << 24)) return fail(787, "sort_rows: row_bytes must be in 1..2^24");
+  if (!num_tokens) return 0;
+  if (!x || !row_of || !valid_rows || !rows) return fail(788, "sort_rows: null pointer");
+  if (x_stride < 0 || (((uintptr_t)row_of | (uintptr_t)valid_rows) & 3)) return fail(789, "sort_rows: negative x_stride or misaligned tables");
+  return cuda_fail(launch_sort_rows(x, x_stride, num_tokens, row_bytes, row_of, top_k, valid_rows, rows, (cudaStream_t)stream), "sort_rows");
+}
+
+static int unsort_checked(const char* what, const UnsortParams& p, const void* other) {
+  if (int rc = order_sizes(what, p.T, p.K)) return rc;
+  if (p.cols <= 0 || p.cols > (1 << 24) || p.n_rows < 0 || p.n_rows > INT32_MAX) return fail(787, "%s: cols must be in 1..2^24, rows below 2^31", what);
+  if (p.dtype < kBf16 || p.dtype > kF32) return fail(787, "%s: unknown dtype", what);
+  if (!p.T) return 0;
+  if (!p.row_of || !p.y) return fail(788, "%s: null pointer", what);
+  const uintptr_t size = p.dtype == kF32 ? 4 : 2;
+  if (p.rows_stride < 0 || p.y_stride < 0) return fail(789, "%s: negative stride", what);
+  if ((((uintptr_t)p.rows | (uintptr_t)p.y | (uintptr_t)other) & (size - 1)) || (((uintptr_t)p.row_of | (uintptr_t)p.weights) & 3))
+    return fail(789, "%s: a tensor is not aligned to its elements", what);
+  return 0;
+}
+
+int b200moe_unsort_rows(const void* rows, int64_t rows_stride, int64_t num_rows, const int32_t* row_of, const float* weights, int64_t num_tokens,
+                        int32_t top_k, int64_t cols, int32_t dtype, void* out, int64_t out_stride, void* stream) {
+  const UnsortParams p{rows, row_of, weights, out, rows_stride, num_rows, out_stride, num_tokens, cols, top_k, dtype};
+  if (int rc = unsort_checked("unsort_rows", p, nullptr)) return rc;
+  if (num_tokens && ((!rows && num_rows) || out_stride < cols)) return fail(788, "unsort_rows: rows is null or out_stride below cols");
+  return cuda_fail(launch_unsort_rows(p, (cudaStream_t)stream), "unsort_rows");
+}
+
+int b200moe_unsort_rows_backward(const void* grad_out, int64_t grad_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
+                                 const float* weights, int64_t num_tokens, int32_t top_k, int64_t cols, int32_t dtype, const int32_t* valid_rows,
+                                 void* grad_rows, float* grad_weights, void* stream) {
+  const UnsortParams p{rows, row_of, weights, const_cast<void*>(grad_out), rows_stride, num_tokens * top_k, grad_stride, num_tokens, cols, top_k, dtype};
+  if (int rc = unsort_checked("unsort_rows_backward", p, grad_rows)) return rc;
+  if (num_tokens && ((grad_rows && !valid_rows) || (grad_weights && !rows))) return fail(788, "unsort_rows_backward: valid_rows or rows is null");
+  if (((uintptr_t)valid_rows | (uintptr_t)grad_weights) & 3) return fail(789, "unsort_rows_backward: a tensor is not aligned to its elements");
+  if (!grad_rows && !grad_weights) return 0;
+  return cuda_fail(launch_unsort_backward(p, valid_rows, grad_rows, grad_weights, (cudaStream_t)stream), "unsort_rows_backward");
+}
+
 int b200moe_route_map_noalloc(const int32_t* ids, const float* weights, int32_t T, int32_t top_k, int32_t num_shared,
                               int32_t num_experts, int32_t offset, int32_t* counts, int32_t* seg_start, int32_t* tile_expert,
                               int32_t* tile_row0, int32_t* tile_rows, int32_t* totals, int32_t* row_of, int32_t* tok_of_row,

@@ -244,6 +244,25 @@ struct Gemm8Params {
 };
 int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
 
+// ---- tokens in the order of their experts, and back (route_order.cu)
+constexpr int kOrderMaxExperts = 1024;
+int64_t route_sort_workspace_bytes(int64_t total, int E);
+int launch_route_sort(const int32_t* ids, int64_t stride, int64_t T, int K, int E, int32_t* offsets, int32_t* row_of, int32_t* route_of_row, void* workspace,
+                      cudaStream_t st);
+// valid: device count of the rows that hold a route; the others become zero. x_stride in bytes.
+int launch_sort_rows(const void* x, int64_t x_stride, int64_t T, int64_t row_bytes, const int32_t* row_of, int K, const int32_t* valid, void* rows,
+                     cudaStream_t st);
+struct UnsortParams {
+  const void* rows;
+  const int32_t* row_of;
+  const float* weights;                      // may be null (= 1)
+  void* y;                                   // [T, cols]; the backward pass reads its gradient here
+  int64_t rows_stride, n_rows, y_stride, T, cols;   // strides in elements
+  int K, dtype;
+};
+int launch_unsort_rows(const UnsortParams& p, cudaStream_t st);
+int launch_unsort_backward(const UnsortParams& p, const int32_t* valid, void* drows, float* dweights, cudaStream_t st);   // drows contiguous
+
 // ---- expert-parallel exchange over peer memory (ep_exchange.cu)
 constexpr int kEpMaxRanks = 16;
 // int32 fields of a rank's control block, each kEpMaxRanks wide and indexed by the peer that writes it

@@ -82,3 +82,47 @@ def test_gemm_8bit_refusals(lib):
     assert abi(a=24) == 783 and abi(b=8) == 783 and abi(a_st=48) == 783 and abi(a_st=72) == 783 and abi(o_st=31) == 783 and abi(out=17) == 783
     assert abi(m=0, a=None) == 0 and abi(e=0, off=16) == 784 and abi(e=1025, off=16) == 784 and abi(e=3) == 786 and abi(e=3, off=18) == 783
     assert abi(e=1024, off=16, n=1 << 21) == 784
+
+
+def test_route_order_refusals(lib):
+    i32 = torch.int32
+    ids = z(4, 2, dtype=i32)
+    order = ks.RouteOrder(z(9, dtype=i32), ids, z(8, dtype=i32))
+    for call in (lambda: ks.route_sort(ids, 8),                                                       # not on a device
+                 lambda: ks.route_sort(ids.long(), 8), lambda: ks.route_sort(ids[0], 8), lambda: ks.route_sort(ids, 0), lambda: ks.route_sort(ids, 1025),
+                 lambda: ks.route_sort(z(4, 0, dtype=i32), 8),
+                 lambda: ks.sort_tokens(z(4, 64), order), lambda: ks.sort_tokens(z(5, 64), order), lambda: ks.sort_tokens(z(4, 64, dtype=torch.float64), order),
+                 lambda: ks.sort_tokens(z(4, 2, 2), order), lambda: ks.sort_tokens(z(4, 0), order),
+                 lambda: ks.sort_tokens(z(4, 64), order._replace(row_of=ids.long())), lambda: ks.sort_tokens(z(4, 64), order._replace(row_of=ids.t())),
+                 lambda: ks.unsort_tokens(z(8, 64), order), lambda: ks.unsort_tokens(z(4, 64), order), lambda: ks.unsort_tokens(z(8, 64, dtype=torch.int8), order),
+                 lambda: ks.unsort_tokens(z(8, 64), order, z(4, 2)), lambda: ks.unsort_tokens(z(8, 64), order, z(2, 4, dtype=torch.float32))):
+        with pytest.raises(ValueError):
+            call()
+
+    size = lib.b200moe_route_sort_workspace_bytes
+    assert size(1024, 8, 128) == 0 and size(1025, 8, 128) == 10 * 129 * 4 and size(1, 1, 1025) == -1 and size(1 << 28, 8, 4) == -1 and size(-1, 8, 4) == -1
+
+    def sort(ids=16, st=8, t=4, k=8, e=16, off=16, row=16, inv=16, ws=None, wb=0):
+        return lib.b200moe_route_sort(ids, st, t, k, e, off, row, inv, ws, wb, None)
+
+    assert sort(t=-1) == 787 and sort(k=0) == 787 and sort(t=1 << 28) == 787 and sort(e=0) == 787 and sort(e=1025) == 787
+    assert sort(ids=None) == 788 and sort(off=None) == 788 and sort(inv=None) == 788 and sort(st=-1) == 789 and sort(row=18) == 789
+    assert sort(t=4096) == 771 and sort(t=4096, ws=16, wb=100) == 771
+
+    def rows(x=16, st=64, t=4, rb=64, row=16, k=2, valid=16, out=16):
+        return lib.b200moe_sort_rows(x, st, t, rb, row, k, valid, out, None)
+
+    assert rows(rb=0) == 787 and rows(t=-1) == 787 and rows(k=0) == 787 and rows(x=None) == 788 and rows(valid=None) == 788 and rows(st=-1) == 789
+    assert rows(row=18) == 789 and rows(t=0, x=None) == 0
+
+    def back(r=16, rs=64, n=8, row=16, w=None, t=4, k=2, c=64, dt=0, out=16, os=64):
+        return lib.b200moe_unsort_rows(r, rs, n, row, w, t, k, c, dt, out, os, None)
+
+    assert back(c=0) == 787 and back(dt=3) == 787 and back(n=-1) == 787 and back(r=None) == 788 and back(row=None) == 788 and back(os=63) == 788
+    assert back(rs=-1) == 789 and back(r=17) == 789 and back(w=18) == 789 and back(t=0, r=None) == 0
+
+    def grad(g=16, gs=64, r=16, rs=64, row=16, w=16, t=4, k=2, c=64, dt=0, valid=16, gr=16, gw=16):
+        return lib.b200moe_unsort_rows_backward(g, gs, r, rs, row, w, t, k, c, dt, valid, gr, gw, None)
+
+    assert grad(c=0) == 787 and grad(g=None) == 788 and grad(valid=None) == 788 and grad(r=None) == 788 and grad(gr=17) == 789 and grad(gw=18) == 789
+    assert grad(gr=None, gw=None) == 0 and grad(t=0) == 0
