@@ -196,7 +196,7 @@ int b200moe_gemm_8bit(const void* a, int64_t a_stride, const float* a_scale, con
                       int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type, int32_t* status, void* stream);
 /* The same over segments of rows, each with its own weights: rows offsets[e] .. offsets[e + 1] - 1 (device int32 [experts + 1], ascending) times
  * b[e] of b [experts, N, K] with b_scale [experts, N]. Segments may be empty. Rows of no segment are left as they are, or become zero
- * with zero_rest. Offsets are cut to 0..M and to ascending order, so no value of theirs reaches memory outside the tensors. experts <= 1024. */
+ * with zero_rest. Offsets are cut to 0..M and to ascending order, so no value of theirs reaches memory outside the tensors. experts <= 1024, M <= 2^27. */
 int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale,
                               const int32_t* offsets, int32_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride,
                               int32_t code, int32_t out_type, int32_t zero_rest, int32_t* status, void* stream);

@@ -728,7 +728,7 @@ int b200moe_gemm_8bit(const void* a, int64_t a_stride, const float* a_scale, con
 int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
                               int32_t experts, void* out, int64_t m, int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type,
                               int32_t zero_rest, int32_t* status, void* stream) {
-  if (experts <= 0 || experts > kGemm8MaxExperts) return fail(784, "gemm_8bit_grouped: need 0 < experts <= %d", kGemm8MaxExperts);
+  if (experts <= 0 || experts > kGemm8MaxExperts || m > (1 << 27)) return fail(784, "gemm_8bit_grouped: need 0 < experts <= %d and M <= 2^27", kGemm8MaxExperts);
   if (m > 0 && !offsets) return fail(786, "gemm_8bit_grouped: offsets is null");
   return gemm_8bit_checked(a, a_stride, a_scale, b, b_scale, offsets, experts, out, m, n, k, out_stride, code, out_type, zero_rest != 0, status, stream);
 }

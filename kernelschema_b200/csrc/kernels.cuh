@@ -242,6 +242,8 @@ struct Gemm8Params {
   int code, out_type;                        // kInt8 / kE4m3; kBf16 / kF16 / kF32
   int zero_rest;                             // grouped: rows of no segment become zero
 };
+// Few tokens (gemm_8bit_decode.cu).
+int launch_gemm_8bit_decode(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
 int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
 
 // ---- tokens in the order of their experts, and back (route_order.cu)

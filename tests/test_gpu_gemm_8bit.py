@@ -44,6 +44,10 @@ def check(out, a, sa, b, sb):
 SHAPES = [(1, 128, 128), (1, 1, 16), (2, 129, 48), (15, 31, 112), (16, 127, 128), (17, 256, 144), (32, 100, 1024), (33, 384, 272), (64, 128, 4096),
           (65, 640, 512), (100, 2113, 528), (128, 96, 1040), (129, 128, 2048), (200, 1000, 640), (255, 130, 256), (256, 512, 400), (257, 77, 1536),
           (300, 4096, 256), (512, 1024, 1024), (1000, 333, 2064), (2049, 256, 768), (3, 4096, 7168), (8, 2048, 16384), (24, 7168, 2048), (1, 20000, 64)]
+# one at least for each form that the library chooses among: few and many tiles of 16, 64 and 128 tokens, K split over 4 and 8 blocks, CTA pairs
+SHAPES += [(1, 18470, 128), (9, 23005, 96), (16, 50, 14016), (5, 1223, 10112), (2, 4480, 3568), (17, 19156, 16), (22, 17, 1552), (627, 1, 2304), (17, 5243, 2896),
+           (655, 1, 16), (666, 3164, 16), (651, 130, 1776), (1233, 20, 1968), (1339, 260, 5632), (1642, 1, 4288), (1642, 300, 4288), (897, 2509, 1344),
+           (2500, 2700, 1040), (19053, 1, 16), (4097, 600, 2064)]
 
 
 @pytest.mark.parametrize("kind", CODES)
