@@ -211,7 +211,7 @@ int64_t b200moe_route_sort_workspace_bytes(int64_t num_tokens, int32_t top_k, in
 int b200moe_route_sort(const int32_t* ids, int64_t ids_stride, int64_t num_tokens, int32_t top_k, int32_t num_experts, int32_t* offsets,
                        int32_t* row_of, int32_t* route_of_row, void* workspace, int64_t workspace_bytes, void* stream);
 /* rows[row_of[t, k]] = x[t], rows of any type as row_bytes bytes (x_stride bytes between tokens); rows [T * top_k] contiguous, zero from
- * *valid_rows (device: the last of the offsets) on. Its gradient is b200moe_unsort_rows without weights. */
+ * *valid_rows (device: the last of the offsets) on. Its gradient is b200moe_unsort_rows without weights. Fewer than 2^26 tokens, here and below. */
 int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64_t row_bytes, const int32_t* row_of, int32_t top_k,
                       const int32_t* valid_rows, void* rows, void* stream);
 /* out[t] = sum_k weights[t, k] * rows[row_of[t, k]] (weights NULL: 1), slots in ascending k, fp32, rounded once; row_of outside 0..num_rows - 1 is

@@ -760,6 +760,7 @@ int b200moe_route_sort(const int32_t* ids, int64_t ids_stride, int64_t num_token
 int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64_t row_bytes, const int32_t* row_of, int32_t top_k,
                       const int32_t* valid_rows, void* rows, void* stream) {
   if (int rc = order_sizes("sort_rows", num_tokens, top_k)) return rc;
+  if (num_tokens >= kOrderMaxTokens) return fail(787, "sort_rows: 2^26 tokens or more are not supported");
   if (row_bytes <= 0 || row_bytes > (1 << 24)) return fail(787, "sort_rows: row_bytes must be in 1..2^24");
   if (!num_tokens) return 0;
   if (!x || !row_of || !valid_rows || !rows) return fail(788, "sort_rows: null pointer");
@@ -769,6 +770,7 @@ int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64
 
 static int unsort_checked(const char* what, const UnsortParams& p, const void* other) {
   if (int rc = order_sizes(what, p.T, p.K)) return rc;
+  if (p.T >= kOrderMaxTokens) return fail(787, "%s: 2^26 tokens or more are not supported", what);
   if (p.cols <= 0 || p.cols > (1 << 24) || p.n_rows < 0 || p.n_rows > INT32_MAX) return fail(787, "%s: cols must be in 1..2^24, rows below 2^31", what);
   if (p.dtype < kBf16 || p.dtype > kF32) return fail(787, "%s: unknown dtype", what);
   if (!p.T) return 0;

@@ -248,6 +248,7 @@ int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8
 
 // ---- tokens in the order of their experts, and back (route_order.cu)
 constexpr int kOrderMaxExperts = 1024;
+constexpr int64_t kOrderMaxTokens = 1 << 26;   // of the row kernels, which count threads in 32 bits
 int64_t route_sort_workspace_bytes(int64_t total, int E);
 int launch_route_sort(const int32_t* ids, int64_t stride, int64_t T, int K, int E, int32_t* offsets, int32_t* row_of, int32_t* route_of_row, void* workspace,
                       cudaStream_t st);

@@ -8,10 +8,8 @@
 //   gradient   drows[row_of[t, k]] = w[t, k] * dy[t], zeros behind offsets[E];  dw[t, k] = <rows[row_of[t, k]], dy[t]>
 //
 // No atomics on global memory, every sum in a fixed order: the same inputs give the same bits.
-#include <cuda_fp16.h>
-
 #include "kernels.cuh"
-#include "ptx.cuh"
+#include "rows.cuh"
 
 namespace b200 {
 
@@ -130,10 +128,15 @@ __global__ void __launch_bounds__(kOrdThreads) k_order_scatter(const OrderView v
     for (int e = threadIdx.x; e < nb; e += kOrdThreads) {
       int sum = 0, mine = 0;
       if (kForm == 1) {
-#pragma unroll 8
-        for (int c = 0; c < chunks; ++c) {
-          if (c == (int)blockIdx.x) mine = sum;
-          sum += __ldg(counts + (int64_t)c * nb + e);
+        for (int c0 = 0; c0 < chunks; c0 += 32) {            // 32 counts in flight: their latency is most of this kernel's time
+          int n[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) n[i] = c0 + i < chunks ? __ldg(counts + (int64_t)(c0 + i) * nb + e) : 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (c0 + i == (int)blockIdx.x) mine = sum;
+            sum += n[i];
+          }
         }
       } else {
         mine = __ldg(counts + (int64_t)blockIdx.x * nb + e);
@@ -188,148 +191,313 @@ __global__ void __launch_bounds__(kOrdThreads) k_order_scatter(const OrderView v
 }
 
 // ----------------------------------------------------------------------------- rows
-DEV float to_f(float v) { return v; }
-DEV float to_f(__half v) { return __half2float(v); }
-DEV float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T>
-DEV T from_f(float v);
-template <>
-DEV float from_f<float>(float v) { return v; }
-template <>
-DEV __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-DEV __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// E elements of T as one access (16 bytes, or one element where rows do not start on 16-byte boundaries).
-template <class T, int E>
-struct __align__(sizeof(T) * E) Piece {
-  T v[E];
-};
-
+// A token's row is `pieces` vectors of 16 bytes. Rows on 16-byte boundaries are read and written as they are. Others (kAny) are cut where the vectors
+// of the row that is WRITTEN lie: its aligned vectors are filled from source vectors that are shifted into place (Any16), and up to 15
+// bytes at either end go element by element, by the first 32 threads of the token.
 constexpr int kRowThreads = 256;
 
-// Zeros in the rows behind the last route: dealt to all threads of the grid.
-template <class P>
-DEV void zero_behind(P* rows, int64_t pieces, const int32_t* valid, int64_t n_rows) {
-  const int64_t first = (int64_t)min(max(__ldg(valid), 0), (int)n_rows) * pieces, end = n_rows * pieces;
-  P zero;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(P) / sizeof(zero.v[0])); ++i) zero.v[i] = decltype(zero.v[0] + zero.v[0])(0);
-  for (int64_t i = first + (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < end; i += (int64_t)gridDim.x * kRowThreads) rows[i] = zero;
+// `lanes` consecutive threads of the grid share a token. The division by lanes is a multiplication (n / d for n < 2^31: Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
+struct Spread {
+  uint32_t lanes, mul, shift;
+  int64_t t;
+  uint32_t lane;
+  DEV void place() {
+    const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x, q = (__umulhi(mul, i) + i) >> shift;
+    t = q;
+    lane = i - q * lanes;
+  }
+};
+
+// How a row of `bytes` that starts at `at` is written: `head` bytes, whole vectors, the rest.
+struct Cut {
+  int head, pieces, tail;
+  DEV Cut(const void* at, int bytes) {
+    head = min((int)(-(uint32_t)(uintptr_t)at & 15u), bytes);
+    pieces = (bytes - head) >> 4;
+    tail = head + 16 * pieces;
+  }
+  // byte of the element that thread `lane` has at the ends, or -1
+  template <class T>
+  DEV int edge(int lane, int bytes) const {
+    if (lane >= 32) return -1;
+    const int b = (lane & 15) * (int)sizeof(T) + (lane < 16 ? 0 : tail);
+    return b < (lane < 16 ? head : bytes) ? b : -1;
+  }
+};
+
+// Zeros in the rows behind the last route, one run of bytes: vectors dealt to all threads of the grid, elements of T at its ends.
+template <class T>
+DEV void zero_behind(uint8_t* rows, int row_bytes, const int32_t* valid, int64_t n_rows) {
+  const int64_t first = min(max((int64_t)__ldg(valid), (int64_t)0), n_rows);
+  if (first == n_rows) return;
+  uint8_t* at = rows + first * row_bytes;
+  const int64_t bytes = (n_rows - first) * row_bytes, head = min((int64_t)(-(uint32_t)(uintptr_t)at & 15u), bytes), pieces = (bytes - head) >> 4;
+  for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * kRowThreads)
+    reinterpret_cast<uint4*>(at + head)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (blockIdx.x == 0 && threadIdx.x < 32) {
+    const int64_t b = (int64_t)(threadIdx.x & 15) * (int)sizeof(T) + (threadIdx.x < 16 ? 0 : head + 16 * pieces);
+    if (b < (threadIdx.x < 16 ? head : bytes)) *reinterpret_cast<T*>(at + b) = 0;
+  }
 }
 
-// A thread owns N pieces of one token (pieces p, p + lanes, ...): read once, written to the token's K rows.
-// `lanes` threads share a token; the grid covers T * lanes threads.
-template <class U, int E, int N>
-__global__ void __launch_bounds__(kRowThreads) k_sort_rows(const U* __restrict__ x, int64_t x_stride, int64_t T, int64_t pieces, int64_t lanes,
+template <class T>
+struct Bits;                 // an unsigned integer as wide as T
+template <>
+struct Bits<__half> { using type = uint16_t; };
+template <>
+struct Bits<__nv_bfloat16> { using type = uint16_t; };
+template <>
+struct Bits<float> { using type = uint32_t; };
+
+// A thread has N pieces of one token, lanes apart: read once, written to the token's K rows (kAny: read for each row, from L1).
+template <class U, int N, bool kAny>
+__global__ void __launch_bounds__(kRowThreads) k_sort_rows(const uint8_t* __restrict__ x, int64_t x_stride, int64_t T, int row_bytes, Spread sp,
                                                            const int32_t* __restrict__ row_of, int K, const int32_t* __restrict__ valid,
-                                                           U* __restrict__ rows) {
-  using P = Piece<U, E>;
+                                                           uint8_t* __restrict__ rows) {
   pdl_trigger();
   pdl_wait();
-  const int64_t n_rows = T * K;
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t t = i / lanes, p0 = i - t * lanes;
+  sp.place();
+  const int64_t n_rows = T * K, t = sp.t;
   if (t < T) {
-    P v[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (p0 + j * lanes < pieces) v[j] = *(reinterpret_cast<const P*>(x + t * x_stride) + p0 + j * lanes);
-    for (int k = 0; k < K; ++k) {
-      const int64_t row = __ldg(row_of + t * K + k);
-      if (row < 0 || row >= n_rows) continue;
-      P* dst = reinterpret_cast<P*>(rows) + row * pieces;
+    const uint8_t* from = x + t * x_stride;
+    const int lane = (int)sp.lane, all = (int)sp.lanes;
+    if constexpr (!kAny) {
+      uint4 v[N];
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (p0 + j * lanes < pieces) dst[p0 + j * lanes] = v[j];
+        if ((lane + j * all) * 16 < row_bytes) v[j] = __ldg(reinterpret_cast<const uint4*>(from) + lane + j * all);
+      for (int k = 0; k < K; ++k) {
+        const int row = __ldg(row_of + t * K + k);
+        if ((uint32_t)row >= (uint64_t)n_rows) continue;
+        uint4* dst = reinterpret_cast<uint4*>(rows + (int64_t)row * row_bytes);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if ((lane + j * all) * 16 < row_bytes) dst[lane + j * all] = v[j];
+      }
+    } else {
+      const Span sx{x, x + (T - 1) * x_stride + row_bytes, from - 15 >= x && from + row_bytes + 32 <= x + (T - 1) * x_stride + row_bytes};
+      for (int k = 0; k < K; ++k) {
+        const int row = __ldg(row_of + t * K + k);
+        if ((uint32_t)row >= (uint64_t)n_rows) continue;
+        uint8_t* dst = rows + (int64_t)row * row_bytes;
+        const Cut cut(dst, row_bytes);
+        for (int i = lane; i < cut.pieces; i += all) {
+          Any16<U> f;
+          f.fetch(from + cut.head + 16 * i, sx, true);
+          reinterpret_cast<uint4*>(dst + cut.head)[i] = f.take(from + cut.head + 16 * i, sx);
+        }
+        const int b = cut.template edge<U>(lane, row_bytes);
+        if (b >= 0) *reinterpret_cast<U*>(dst + b) = *reinterpret_cast<const U*>(from + b);
+      }
     }
   }
-  zero_behind(reinterpret_cast<P*>(rows), pieces, valid, n_rows);
+  zero_behind<U>(rows, row_bytes, valid, n_rows);
 }
 
-// y[t] (+ weights): eight slots' rows in flight per thread, one piece of a token each.
-template <class T_, int E>
-__global__ void __launch_bounds__(kRowThreads) k_unsort_rows(const T_* __restrict__ rows, int64_t rows_stride, int64_t n_rows,
-                                                             const int32_t* __restrict__ row_of, const float* __restrict__ weights, int64_t T, int K,
-                                                             int64_t pieces, T_* __restrict__ y, int64_t y_stride) {
-  using P = Piece<T_, E>;
+// The span of a tensor for each of its rows: every row but the first and the last has its neighbours around it.
+template <class T>
+struct RowSpans {
+  const uint8_t *lo, *hi;
+  int64_t last;
+  DEV RowSpans(const void* p, int64_t rows, int64_t stride, int64_t cols) {
+    lo = (const uint8_t*)p;
+    hi = lo + ((rows - 1) * stride + cols) * (int64_t)sizeof(T);
+    last = stride >= cols && cols * (int64_t)sizeof(T) >= 32 ? rows - 1 : 0;
+  }
+  DEV Span of(int64_t row) const { return {lo, hi, row > 0 && row < last}; }
+};
+
+// Rows of a few elements (scales): a thread per route.
+template <class U>
+__global__ void __launch_bounds__(kRowThreads) k_sort_short(const uint8_t* __restrict__ x, int64_t x_stride, int64_t T, int row_bytes,
+                                                            const int32_t* __restrict__ row_of, int K, const int32_t* __restrict__ valid,
+                                                            uint8_t* __restrict__ rows) {
   pdl_trigger();
   pdl_wait();
-  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t t = i / pieces, p = i - t * pieces;
-  if (t >= T) return;
-  float acc[E];
+  const int64_t n_rows = T * K, i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i < n_rows) {
+    const int row = __ldg(row_of + i);
+    const uint8_t* from = x + (int64_t)((uint32_t)i / (uint32_t)K) * x_stride;
+    if ((uint32_t)row < (uint64_t)n_rows)
+      for (int b = 0; b < row_bytes; b += (int)sizeof(U)) *reinterpret_cast<U*>(rows + (int64_t)row * row_bytes + b) = __ldg(reinterpret_cast<const U*>(from + b));
+  }
+  zero_behind<U>(rows, row_bytes, valid, n_rows);
+}
+
+// Rows and weights of up to S slots.
+template <int S>
+struct Slots {
+  int row[S];
+  float w[S];
+  DEV Slots(const int32_t* row_of, const float* weights, int64_t t, int K, int k0, int64_t n_rows) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int k0 = 0; k0 < K; k0 += 8) {
-    int64_t row[8];
-    float w[8];
-    P v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < S; ++j) {
       row[j] = k0 + j < K ? __ldg(row_of + t * K + k0 + j) : -1;
       w[j] = weights && k0 + j < K ? __ldg(weights + t * K + k0 + j) : 1.f;
-      if (row[j] >= n_rows) row[j] = -1;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (row[j] >= 0) v[j] = *(reinterpret_cast<const P*>(rows + row[j] * rows_stride) + p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (row[j] >= 0) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(to_f(v[j].v[e]), w[j], acc[e]);
-      }
+    for (int j = 0; j < S; ++j)
+      if ((uint32_t)row[j] >= (uint64_t)n_rows) row[j] = -1;
   }
-  P o;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o.v[e] = from_f<T_>(acc[e]);
-  *(reinterpret_cast<P*>(y + t * y_stride) + p) = o;
-}
+};
 
-// One warp per token: a piece of dy is read once for the token's K rows; their dot products stay in registers, four slots at a time.
-template <class T_, int E>
-__global__ void __launch_bounds__(kRowThreads) k_unsort_backward(const T_* __restrict__ dy, int64_t dy_stride, const T_* __restrict__ rows,
-                                                                 int64_t rows_stride, const int32_t* __restrict__ row_of,
-                                                                 const float* __restrict__ weights, int64_t T, int K, int64_t pieces,
-                                                                 const int32_t* __restrict__ valid, T_* __restrict__ drows, float* __restrict__ dweights) {
-  using P = Piece<T_, E>;
-  constexpr int kSlots = 4;
+// y[t]: a thread has N pieces of a token, and the rows of S slots in flight for them: eight vectors, or four that are shifted.
+template <class T_, int S, int N, bool kAny>
+__global__ void __launch_bounds__(kRowThreads) k_unsort_rows(const UnsortParams p, Spread sp) {
+  constexpr int E = Vec<T_>::E;
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5), n_rows = T * K;
-  if (t < T) {
-    for (int k0 = 0; k0 < K; k0 += kSlots) {
-      int64_t row[kSlots];
+  sp.place();
+  const int64_t t = sp.t;
+  if (t >= p.T) return;
+  const T_* rows = (const T_*)p.rows;
+  T_* y = (T_*)p.y + t * p.y_stride;
+  const int lane = (int)sp.lane, all = (int)sp.lanes, bytes = (int)p.cols * (int)sizeof(T_);
+  const Cut cut = kAny ? Cut(y, bytes) : Cut(nullptr, bytes);
+  const RowSpans<T_> sr(p.rows, p.n_rows, p.rows_stride, p.cols);
+  for (int i = lane; i < cut.pieces; i += N * all) {
+    float acc[N][E];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
+    for (int k0 = 0; k0 < p.K; k0 += S) {
+      const Slots<S> s(p.row_of, p.weights, t, p.K, k0, p.n_rows);
+      Fetch16<T_, kAny> f[S][N];
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int at = i + n * all;
+          f[j][n].fetch(reinterpret_cast<const uint8_t*>(rows + (int64_t)max(s.row[j], 0) * p.rows_stride) + cut.head + 16 * at,
+                        sr.of(s.row[j]), s.row[j] >= 0 && (N == 1 || at < cut.pieces));
+        }
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        if (s.row[j] < 0) continue;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          Vec<T_> v;
+          v.raw = f[j][n].take(reinterpret_cast<const uint8_t*>(rows + (int64_t)s.row[j] * p.rows_stride) + cut.head + 16 * (i + n * all), sr.of(s.row[j]));
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[n][e] = fmaf(to_f32(v.v[e]), s.w[j], acc[n][e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int at = i + n * all;
+      if (N > 1 && at >= cut.pieces) continue;
+      Vec<T_> o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = from_f32<T_>(acc[n][e]);
+      reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(y) + cut.head)[at] = o.raw;
+    }
+  }
+  if constexpr (kAny) {
+    const int b = cut.template edge<T_>(lane, bytes);
+    if (b >= 0) {
+      const int c = b / (int)sizeof(T_);
+      float acc = 0.f;
+      for (int k0 = 0; k0 < p.K; k0 += S) {
+        const Slots<S> s(p.row_of, p.weights, t, p.K, k0, p.n_rows);
+        T_ v[S];
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = s.row[j] >= 0 ? rows[(int64_t)s.row[j] * p.rows_stride + c] : from_f32<T_>(0.f);
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+          if (s.row[j] >= 0) acc = fmaf(to_f32(v[j]), s.w[j], acc);
+      }
+      y[c] = from_f32<T_>(acc);
+    }
+  }
+}
+
+// One warp per token, or one block (kBlock: few tokens with long rows). A piece of dy is read once for four of the token's rows; their dot
+// products stay in registers until the row's end.
+template <class T_, bool kAny, bool kBlock>
+__global__ void __launch_bounds__(kRowThreads) k_unsort_backward(const UnsortParams p, const int32_t* __restrict__ valid, T_* __restrict__ drows,
+                                                                 float* __restrict__ dweights) {
+  constexpr int E = Vec<T_>::E, kSlots = 4, kWarps = kRowThreads / 32;
+  __shared__ float part[kWarps][kSlots];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5;
+  const int lane = kBlock ? (int)threadIdx.x : (int)threadIdx.x & 31, all = kBlock ? kRowThreads : 32;
+  const int64_t t = kBlock ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarps + warp;
+  const int bytes = (int)p.cols * (int)sizeof(T_);
+  const T_* rows = (const T_*)p.rows;
+  const T_* dy = (const T_*)p.y + t * p.y_stride;
+  const RowSpans<T_> rows_of(p.rows, p.n_rows, p.rows_stride, p.cols), grads_of(p.y, p.T, p.y_stride, p.cols);
+  const Span sd = grads_of.of(t);
+  if (t < p.T) {
+    for (int k0 = 0; k0 < p.K; k0 += kSlots) {
+      int row[kSlots];
       float w[kSlots], dot[kSlots];
 #pragma unroll
       for (int j = 0; j < kSlots; ++j) {
-        row[j] = k0 + j < K ? __ldg(row_of + t * K + k0 + j) : -1;
-        w[j] = weights && k0 + j < K ? __ldg(weights + t * K + k0 + j) : 1.f;
-        if (row[j] >= n_rows) row[j] = -1;
+        row[j] = k0 + j < p.K ? __ldg(p.row_of + t * p.K + k0 + j) : -1;
+        w[j] = p.weights && k0 + j < p.K ? __ldg(p.weights + t * p.K + k0 + j) : 1.f;
+        if ((uint32_t)row[j] >= (uint64_t)p.n_rows) row[j] = -1;
         dot[j] = 0.f;
       }
-      for (int64_t p = lane; p < pieces; p += 32) {
-        const P g = *(reinterpret_cast<const P*>(dy + t * dy_stride) + p);
-        P v[kSlots];
-        if (dweights) {
+      if constexpr (!kAny) {
+        for (int i = lane; i * 16 < bytes; i += all) {
+          Vec<T_> g, v[kSlots];
+          g.raw = __ldg(reinterpret_cast<const uint4*>(dy) + i);
+          if (dweights) {
 #pragma unroll
-          for (int j = 0; j < kSlots; ++j)
-            if (row[j] >= 0) v[j] = *(reinterpret_cast<const P*>(rows + row[j] * rows_stride) + p);
+            for (int j = 0; j < kSlots; ++j)
+              if (row[j] >= 0) v[j].raw = __ldg(reinterpret_cast<const uint4*>(rows + (int64_t)row[j] * p.rows_stride) + i);
+          }
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            if (row[j] < 0) continue;
+            if (dweights) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) dot[j] = fmaf(to_f32(v[j].v[e]), to_f32(g.v[e]), dot[j]);
+            }
+            if (drows) {
+              Vec<T_> o;
+#pragma unroll
+              for (int e = 0; e < E; ++e) o.v[e] = from_f32<T_>(to_f32(g.v[e]) * w[j]);
+              reinterpret_cast<uint4*>(drows + (int64_t)row[j] * p.cols)[i] = o.raw;
+            }
+          }
         }
+      } else {
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           if (row[j] < 0) continue;
-          if (dweights) {
+          uint8_t* dst = reinterpret_cast<uint8_t*>(drows + (int64_t)row[j] * p.cols);        // its phase, without gradients of rows as well
+          const uint8_t *from = reinterpret_cast<const uint8_t*>(rows + (int64_t)row[j] * p.rows_stride), *grad = reinterpret_cast<const uint8_t*>(dy);
+          const Cut cut(dst, bytes);
+          const Span sr = rows_of.of(row[j]);
+          for (int i = lane; i < cut.pieces; i += all) {
+            const int at = cut.head + 16 * i;
+            Any16<T_> fg, fv;
+            fg.fetch(grad + at, sd, true);
+            fv.fetch(from + at, sr, dweights);
+            Vec<T_> g, v, o;
+            g.raw = fg.take(grad + at, sd);
+            if (dweights) {
+              v.raw = fv.take(from + at, sr);
 #pragma unroll
-            for (int e = 0; e < E; ++e) dot[j] = fmaf(to_f(v[j].v[e]), to_f(g.v[e]), dot[j]);
+              for (int e = 0; e < E; ++e) dot[j] = fmaf(to_f32(v.v[e]), to_f32(g.v[e]), dot[j]);
+            }
+            if (drows) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) o.v[e] = from_f32<T_>(to_f32(g.v[e]) * w[j]);
+              *reinterpret_cast<uint4*>(dst + at) = o.raw;
+            }
           }
-          if (drows) {
-            P o;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o.v[e] = from_f<T_>(to_f(g.v[e]) * w[j]);
-            reinterpret_cast<P*>(drows)[row[j] * pieces + p] = o;
+          const int b = cut.template edge<T_>(lane, bytes);
+          if (b >= 0) {
+            const int c = b / (int)sizeof(T_);
+            const float g = to_f32(dy[c]);
+            if (dweights) dot[j] = fmaf(to_f32(rows[(int64_t)row[j] * p.rows_stride + c]), g, dot[j]);
+            if (drows) drows[(int64_t)row[j] * p.cols + c] = from_f32<T_>(g * w[j]);
           }
         }
       }
@@ -338,40 +506,83 @@ __global__ void __launch_bounds__(kRowThreads) k_unsort_backward(const T_* __res
         for (int j = 0; j < kSlots; ++j) {
 #pragma unroll
           for (int o = 16; o; o >>= 1) dot[j] += __shfl_xor_sync(0xFFFFFFFFu, dot[j], o);
-          if (lane == 0 && k0 + j < K) dweights[t * K + k0 + j] = row[j] >= 0 ? dot[j] : 0.f;
+        }
+        if constexpr (kBlock) {
+          __syncthreads();
+          if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+            for (int j = 0; j < kSlots; ++j) part[warp][j] = dot[j];
+          }
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j) {
+            dot[j] = part[0][j];
+#pragma unroll
+            for (int i = 1; i < kWarps; ++i) dot[j] += part[i][j];
+          }
+        }
+        if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < kSlots; ++j)
+            if (k0 + j < p.K) dweights[t * p.K + k0 + j] = row[j] >= 0 ? dot[j] : 0.f;
         }
       }
     }
   }
-  if (drows) zero_behind(reinterpret_cast<P*>(drows), pieces, valid, n_rows);
+  if (drows) zero_behind<typename Bits<T_>::type>(reinterpret_cast<uint8_t*>(drows), bytes, valid, p.n_rows);
 }
 
 unsigned blocks_of(int64_t n, int64_t per) { return (unsigned)((n + per - 1) / per); }
 
-template <class U, int E>
-int launch_sort(const void* x, int64_t x_stride_bytes, int64_t T, int64_t row_bytes, const int32_t* row_of, int K, const int32_t* valid, void* rows,
-                cudaStream_t st) {
-  const int64_t pieces = row_bytes / (int64_t)(sizeof(U) * E), stride = x_stride_bytes / (int64_t)sizeof(U);
+// `threads` for each of T tokens, fewer where the grid's threads would pass 2^31 (a thread then takes more pieces).
+Spread spread(int64_t threads, int64_t T) {
+  while (threads > 32 && threads * T > INT32_MAX - kRowThreads) threads = (threads + 1) / 2;
+  Spread s{};
+  s.lanes = (uint32_t)threads;
+  while ((1ull << s.shift) < (uint64_t)threads) ++s.shift;
+  s.mul = (uint32_t)(((1ull << 32) * ((1ull << s.shift) - (uint64_t)threads)) / (uint64_t)threads + 1);
+  return s;
+}
+dim3 grid_of(const Spread& s, int64_t T) { return dim3(blocks_of(T * s.lanes, kRowThreads)); }
+
+template <class U, bool kAny>
+int launch_sort(const void* x, int64_t x_stride, int64_t T, int row_bytes, const int32_t* row_of, int K, const int32_t* valid, void* rows, cudaStream_t st) {
+  if (kAny && row_bytes < 32)
+    return (int)launch_chain(k_sort_short<U>, dim3(blocks_of(T * K, kRowThreads)), dim3(kRowThreads), 0, st, (const uint8_t*)x, x_stride, T, row_bytes, row_of, K,
+                             valid, (uint8_t*)rows);
+  const int64_t pieces = (row_bytes + 15) / 16;
   // four pieces per thread once that still fills the device: fewer index reads for the same bytes
   const bool four = T * pieces >= 4ll * 1024 * sm_count();
-  const int64_t lanes = four ? (pieces + 3) / 4 : pieces;
-  const dim3 grid(blocks_of(T * lanes, kRowThreads)), block(kRowThreads);
-  if (four) return (int)launch_chain(k_sort_rows<U, E, 4>, grid, block, 0, st, (const U*)x, stride, T, pieces, lanes, row_of, K, valid, (U*)rows);
-  return (int)launch_chain(k_sort_rows<U, E, 1>, grid, block, 0, st, (const U*)x, stride, T, pieces, lanes, row_of, K, valid, (U*)rows);
+  const int64_t want = four ? (pieces + 3) / 4 : pieces;
+  const Spread sp = spread(kAny && want < 32 ? 32 : want, T);
+  const auto kern = four && !kAny ? k_sort_rows<U, 4, kAny> : k_sort_rows<U, 1, kAny>;
+  return (int)launch_chain(kern, grid_of(sp, T), dim3(kRowThreads), 0, st, (const uint8_t*)x, x_stride, T, row_bytes, sp, row_of, K, valid, (uint8_t*)rows);
 }
 
-template <class T_, int E>
+template <class T_, int S, int N, bool kAny>
+int launch_unsort_form(const UnsortParams& p, cudaStream_t st) {
+  const int64_t pieces = (p.cols * (int64_t)sizeof(T_) / 16 + N - 1) / N;
+  const Spread sp = spread(kAny && pieces < 32 ? 32 : pieces, p.T);
+  return (int)launch_chain(k_unsort_rows<T_, S, N, kAny>, grid_of(sp, p.T), dim3(kRowThreads), 0, st, p, sp);
+}
+// Few slots: more pieces per thread for the same bytes in flight, while that leaves the device full.
+template <class T_, bool kAny>
 int launch_unsort(const UnsortParams& p, cudaStream_t st) {
-  const int64_t pieces = p.cols / E;
-  return (int)launch_chain(k_unsort_rows<T_, E>, dim3(blocks_of(p.T * pieces, kRowThreads)), dim3(kRowThreads), 0, st, (const T_*)p.rows, p.rows_stride,
-                           p.n_rows, p.row_of, p.weights, p.T, p.K, pieces, (T_*)p.y, p.y_stride);
+  if constexpr (kAny) {
+    return launch_unsort_form<T_, 4, 1, true>(p, st);
+  } else {
+    const bool full = p.T * p.cols * (int64_t)sizeof(T_) / 16 >= 8ll * 1024 * sm_count();
+    if (p.K > 4 || !full) return launch_unsort_form<T_, 8, 1, false>(p, st);
+    return p.K > 2 ? launch_unsort_form<T_, 4, 2, false>(p, st) : launch_unsort_form<T_, 2, 4, false>(p, st);
+  }
 }
 
-template <class T_, int E>
+template <class T_, bool kAny>
 int launch_unsort_back(const UnsortParams& p, const int32_t* valid, void* drows, float* dweights, cudaStream_t st) {
-  const int64_t pieces = p.cols / E;
-  return (int)launch_chain(k_unsort_backward<T_, E>, dim3(blocks_of(p.T, kRowThreads / 32)), dim3(kRowThreads), 0, st, (const T_*)p.y, p.y_stride,
-                           (const T_*)p.rows, p.rows_stride, p.row_of, p.weights, p.T, p.K, pieces, valid, (T_*)drows, dweights);
+  // a block per token while warps would leave most of the device idle
+  if (p.T < 16ll * sm_count() && p.cols * (int64_t)sizeof(T_) >= 1024)
+    return (int)launch_chain(k_unsort_backward<T_, kAny, true>, dim3((unsigned)p.T), dim3(kRowThreads), 0, st, p, valid, (T_*)drows, dweights);
+  return (int)launch_chain(k_unsort_backward<T_, kAny, false>, dim3(blocks_of(p.T, kRowThreads / 32)), dim3(kRowThreads), 0, st, p, valid, (T_*)drows, dweights);
 }
 
 bool on16(const void* p, int64_t stride_bytes) { return (((uintptr_t)p | (uintptr_t)stride_bytes) & 15) == 0; }
@@ -411,28 +622,28 @@ int launch_sort_rows(const void* x, int64_t x_stride, int64_t T, int64_t row_byt
                      cudaStream_t st) {
   if (!T || !row_bytes) return 0;
   const uintptr_t all = (uintptr_t)x | (uintptr_t)rows | (uintptr_t)x_stride | (uintptr_t)row_bytes;
-  if (all % 16 == 0) return launch_sort<uint32_t, 4>(x, x_stride, T, row_bytes, row_of, K, valid, rows, st);
-  if (all % 4 == 0) return launch_sort<uint32_t, 1>(x, x_stride, T, row_bytes, row_of, K, valid, rows, st);
-  if (all % 2 == 0) return launch_sort<uint16_t, 1>(x, x_stride, T, row_bytes, row_of, K, valid, rows, st);
-  return launch_sort<uint8_t, 1>(x, x_stride, T, row_bytes, row_of, K, valid, rows, st);
+  if (all % 16 == 0) return launch_sort<uint32_t, false>(x, x_stride, T, (int)row_bytes, row_of, K, valid, rows, st);
+  if (all % 4 == 0) return launch_sort<uint32_t, true>(x, x_stride, T, (int)row_bytes, row_of, K, valid, rows, st);
+  if (all % 2 == 0) return launch_sort<uint16_t, true>(x, x_stride, T, (int)row_bytes, row_of, K, valid, rows, st);
+  return launch_sort<uint8_t, true>(x, x_stride, T, (int)row_bytes, row_of, K, valid, rows, st);
 }
 
 int launch_unsort_rows(const UnsortParams& p, cudaStream_t st) {
   if (!p.T || !p.cols) return 0;
   const int64_t size = p.dtype == kF32 ? 4 : 2;
   const bool vec = p.cols * size % 16 == 0 && on16(p.rows, p.rows_stride * size) && on16(p.y, p.y_stride * size);
-  if (p.dtype == kBf16) return vec ? launch_unsort<__nv_bfloat16, 8>(p, st) : launch_unsort<__nv_bfloat16, 1>(p, st);
-  if (p.dtype == kF16) return vec ? launch_unsort<__half, 8>(p, st) : launch_unsort<__half, 1>(p, st);
-  return vec ? launch_unsort<float, 4>(p, st) : launch_unsort<float, 1>(p, st);
+  if (p.dtype == kBf16) return vec ? launch_unsort<__nv_bfloat16, false>(p, st) : launch_unsort<__nv_bfloat16, true>(p, st);
+  if (p.dtype == kF16) return vec ? launch_unsort<__half, false>(p, st) : launch_unsort<__half, true>(p, st);
+  return vec ? launch_unsort<float, false>(p, st) : launch_unsort<float, true>(p, st);
 }
 
 int launch_unsort_backward(const UnsortParams& p, const int32_t* valid, void* drows, float* dweights, cudaStream_t st) {
   if (!p.T || !p.cols) return 0;
   const int64_t size = p.dtype == kF32 ? 4 : 2;
   const bool vec = p.cols * size % 16 == 0 && on16(p.rows, p.rows_stride * size) && on16(p.y, p.y_stride * size) && on16(drows, 0);
-  if (p.dtype == kBf16) return vec ? launch_unsort_back<__nv_bfloat16, 8>(p, valid, drows, dweights, st) : launch_unsort_back<__nv_bfloat16, 1>(p, valid, drows, dweights, st);
-  if (p.dtype == kF16) return vec ? launch_unsort_back<__half, 8>(p, valid, drows, dweights, st) : launch_unsort_back<__half, 1>(p, valid, drows, dweights, st);
-  return vec ? launch_unsort_back<float, 4>(p, valid, drows, dweights, st) : launch_unsort_back<float, 1>(p, valid, drows, dweights, st);
+  if (p.dtype == kBf16) return vec ? launch_unsort_back<__nv_bfloat16, false>(p, valid, drows, dweights, st) : launch_unsort_back<__nv_bfloat16, true>(p, valid, drows, dweights, st);
+  if (p.dtype == kF16) return vec ? launch_unsort_back<__half, false>(p, valid, drows, dweights, st) : launch_unsort_back<__half, true>(p, valid, drows, dweights, st);
+  return vec ? launch_unsort_back<float, false>(p, valid, drows, dweights, st) : launch_unsort_back<float, true>(p, valid, drows, dweights, st);
 }
 
 }  // namespace b200

@@ -112,13 +112,13 @@ def test_route_order_refusals(lib):
     def rows(x=16, st=64, t=4, rb=64, row=16, k=2, valid=16, out=16):
         return lib.b200moe_sort_rows(x, st, t, rb, row, k, valid, out, None)
 
-    assert rows(rb=0) == 787 and rows(t=-1) == 787 and rows(k=0) == 787 and rows(x=None) == 788 and rows(valid=None) == 788 and rows(st=-1) == 789
+    assert rows(t=1 << 26) == 787 and rows(rb=0) == 787 and rows(t=-1) == 787 and rows(k=0) == 787 and rows(x=None) == 788 and rows(valid=None) == 788 and rows(st=-1) == 789
     assert rows(row=18) == 789 and rows(t=0, x=None) == 0
 
     def back(r=16, rs=64, n=8, row=16, w=None, t=4, k=2, c=64, dt=0, out=16, os=64):
         return lib.b200moe_unsort_rows(r, rs, n, row, w, t, k, c, dt, out, os, None)
 
-    assert back(c=0) == 787 and back(dt=3) == 787 and back(n=-1) == 787 and back(r=None) == 788 and back(row=None) == 788 and back(os=63) == 788
+    assert back(t=1 << 26) == 787 and back(c=0) == 787 and back(dt=3) == 787 and back(n=-1) == 787 and back(r=None) == 788 and back(row=None) == 788 and back(os=63) == 788
     assert back(rs=-1) == 789 and back(r=17) == 789 and back(w=18) == 789 and back(t=0, r=None) == 0
 
     def grad(g=16, gs=64, r=16, rs=64, row=16, w=16, t=4, k=2, c=64, dt=0, valid=16, gr=16, gw=16):
