@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200moe.so")
 SHIM = os.path.join(HERE, "_b200moe_shim.so")
+TORCH_CALLS = os.path.join(HERE, "_b200moe_torch.so")
 SOURCES = ["quantize.cu", "router.cu", "route_map.cu", "gather.cu", "finalize.cu", "gemm_nvfp4.cu", "gemm_w4a16.cu", "gemm_w4a16_decode.cu", "gemm_w4a16_expand.cu", "ep_exchange.cu", "rowquant.cu", "gemm_8bit.cu", "gemm_8bit_decode.cu", "route_order.cu", "api.cu"]
 HEADERS = ["kernels.cuh", "ptx.cuh", "quantize.cuh", "rows.cuh", "topk.cuh", "w4a16.cuh", os.path.join("..", "..", "include", "b200moe.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -62,6 +63,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if res.returncode != 0:
             raise RuntimeError("link failed:\n" + res.stderr)
     build_shim(force)
+    build_torch_calls(force)
     return LIB
 
 
@@ -77,6 +79,24 @@ def build_shim(force: bool = False) -> str:
         if res.returncode != 0:
             raise RuntimeError("shim build failed:\n" + res.stderr)
     return SHIM
+
+
+def build_torch_calls(force: bool = False) -> str:
+    """Compile the calls on torch tensors (C++ against torch's headers; links the in-tree libb200moe.so through $ORIGIN)."""
+    src = os.path.join(CSRC, "torch_calls.cpp")
+    if force or _stale(TORCH_CALLS, [src, LIB, os.path.join(CSRC, "..", "..", "include", "b200moe.h")]):
+        import sysconfig
+        import torch
+        base = os.path.dirname(torch.__file__)
+        cuda = os.path.dirname(os.path.dirname(_nvcc()))
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+               "-I", os.path.join(base, "include"), "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I",
+               os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", TORCH_CALLS, "-L", HERE, "-lb200moe", "-L",
+               os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("build of the torch calls failed:\n" + res.stderr)
+    return TORCH_CALLS
 
 
 if __name__ == "__main__":

@@ -26,6 +26,22 @@ def _shim():
     return _shim_mod
 
 
+_calls_mod = None
+
+
+def _calls():
+    """The calls on torch tensors (built next to the library by ``python -m kernelschema_b200.build``)."""
+    global _calls_mod
+    if _calls_mod is None:
+        _lib.load()
+        try:
+            from . import _b200moe_torch
+        except ImportError as exc:
+            raise RuntimeError("kernelschema_b200/_b200moe_torch.so is missing or of another torch: run `python -m kernelschema_b200.build`") from exc
+        _calls_mod = _b200moe_torch
+    return _calls_mod
+
+
 def _stream() -> int:
     """Handle of the current device's current stream (`torch.cuda.current_stream()` builds a Stream object: 5.4 us a call)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -224,40 +240,6 @@ def mm_bf16_nvfp4(a: torch.Tensor, b: torch.Tensor, b_descale: torch.Tensor, alp
     return out
 
 
-_ROW_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16, torch.float32: _lib.FP32}
-_CODE_TYPES = {torch.int8: _lib.INT8, torch.float8_e4m3fn: _lib.E4M3}
-
-
-def _here(*tensors) -> None:
-    """The tensors of a call are on the current device, whose current stream it uses."""
-    for t in tensors:
-        if t is not None:
-            at = t.get_device()
-            if at < 0:
-                raise ValueError("libb200moe operates on CUDA tensors only")
-            if at != torch._C._cuda_getDevice():
-                raise ValueError(f"a tensor is on cuda:{at}, the current device is cuda:{torch._C._cuda_getDevice()}: call under torch.cuda.device({at})")
-
-
-def _unit_rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    """Elements between rows; a single row has no next one, whatever its stride says."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-
-
-def _out_rows(out, shape, dtype, name: str, device) -> torch.Tensor:
-    """A caller's buffer for rows of `shape`, checked, or a new one."""
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if out.dtype != dtype or tuple(out.shape) != tuple(shape) or (out.dim() == 2 and (out.shape[1] > 1 and out.stride(1) != 1 or _row_stride(out) < shape[1])) \
-            or (out.dim() == 1 and not out.is_contiguous()):
-        raise ValueError(f"{name} must be {dtype} {tuple(shape)} with unit inner stride and rows that do not overlap")
-    return out
-
-
 def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
                      dtype: torch.dtype = torch.int8, normed: bool = False, out=None):
     """Residual addition, RMS norm and 8-bit quantisation of rows in one pass -> (q, scale, hidden, normed).
@@ -268,101 +250,29 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     scale, hidden, normed): caller-owned buffers, each may be None; hidden may be x or residual themselves (in place).
     h and the sums are fp32, and h is not rounded before the norm. A row of zeros (max|y| < 2^-116) has scale 0; a row with a NaN or an infinity, or whose
     squares' sum leaves fp32, has scale NaN and codes 0."""
-    if x.dim() != 2 or x.dtype not in _ROW_TYPES or (residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape)):
-        raise ValueError("rmsnorm_quantize expects bf16, fp16 or fp32 [T, H] and a residual like it")
-    if weight.dim() != 1 or weight.shape[0] != x.shape[1] or weight.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"weight must be [{x.shape[1]}] in x's type or float32")
-    if dtype not in _CODE_TYPES:
-        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
-    q, scale, hidden, norm = out if out is not None else (None, None, None, None)
-    _here(x, weight, residual, q, scale, hidden, norm)
-    x, weight = _unit_rows(x), weight.contiguous()
-    residual = None if residual is None else _unit_rows(residual)
-    t, h = x.shape
-    q = _out_rows(q, (t, h), dtype, "q", x.device)
-    scale = _out_rows(scale, (t,), torch.float32, "scale", x.device)
-    if residual is not None or hidden is not None:
-        hidden = _out_rows(hidden, (t, h), x.dtype, "hidden", x.device)
-    if normed or norm is not None:
-        norm = _out_rows(norm, (t, h), x.dtype, "normed", x.device)
-    _lib.check(_lib.load().b200moe_rmsnorm_quantize(
-        x.data_ptr(), _row_stride(x), _ptr(residual), 0 if residual is None else _row_stride(residual), weight.data_ptr(), _ROW_TYPES[weight.dtype], t, h,
-        eps, _ROW_TYPES[x.dtype], _CODE_TYPES[dtype], q.data_ptr(), _row_stride(q), scale.data_ptr(), _ptr(hidden), 0 if hidden is None else _row_stride(hidden),
-        _ptr(norm), 0 if norm is None else _row_stride(norm), _stream()), "b200moe_rmsnorm_quantize")
-    return q, scale, x if hidden is None else hidden, norm
+    return _calls().rmsnorm_quantize(x, weight, residual, eps, dtype, normed, *(out or (None, None, None, None)))
 
 
 def swiglu_quantize(x: torch.Tensor, dtype: torch.dtype = torch.int8, out=None):
     """x = [gate | up] (bf16, fp16 or fp32 [T, 2I], I <= 32768) -> (q [T, I], scale fp32 [T]) of gate * sigmoid(gate) * up: the step between the two 8-bit
     products of a feed-forward layer or an expert. dtype, scales, special rows and ``out`` = (q, scale) as in `rmsnorm_quantize`."""
-    if x.dim() != 2 or x.dtype not in _ROW_TYPES or x.shape[1] % 2 or not x.shape[1]:
-        raise ValueError("swiglu_quantize expects bf16, fp16 or fp32 [T, 2I]")
-    if dtype not in _CODE_TYPES:
-        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
-    q, scale = out if out is not None else (None, None)
-    _here(x, q, scale)
-    x = _unit_rows(x)
-    t, i = x.shape[0], x.shape[1] // 2
-    q = _out_rows(q, (t, i), dtype, "q", x.device)
-    scale = _out_rows(scale, (t,), torch.float32, "scale", x.device)
-    _lib.check(_lib.load().b200moe_swiglu_quantize(x.data_ptr(), _row_stride(x), t, i, _ROW_TYPES[x.dtype], _CODE_TYPES[dtype], q.data_ptr(),
-                                                   _row_stride(q), scale.data_ptr(), _stream()), "b200moe_swiglu_quantize")
-    return q, scale
-
-
-def _mm_8bit_args(a, a_scale, b, b_scale, lead, out, out_dtype, status, offsets=None):
-    """Checks that `mm_8bit` (lead = ()) and `mm_8bit_grouped` (lead = (experts,)) share -> (a, a_scale, b, b_scale, out)."""
-    if a.dim() != 2 or b.dim() != 2 + len(lead) or a.dtype not in _CODE_TYPES or b.dtype != a.dtype:
-        raise ValueError("a [M, K] and b [N, K] (experts: [E, N, K]) must both be int8 or both float8_e4m3fn")
-    m, k = a.shape
-    n = b.shape[-2]
-    if b.shape[-1] != k or k % 16 or not k or not n:
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} must share K, a multiple of 16")
-    if a_scale.dtype != torch.float32 or a_scale.numel() != m or b_scale.dtype != torch.float32 or b_scale.numel() != b.numel() // k:
-        raise ValueError("a_scale must hold one fp32 value per row of a, b_scale one per row of b")
-    if out_dtype not in _ROW_TYPES:
-        raise ValueError("out_dtype must be bfloat16, float16 or float32")
-    if status is not None and (status.dtype != torch.int32 or not status.numel()):
-        raise ValueError("status must be an int32 tensor")
-    _here(a, a_scale, b, b_scale, out, status, offsets)
-    a = _unit_rows(a)
-    if _row_stride(a) % 16 or a.data_ptr() % 16:
-        a = a.contiguous() if not a.is_contiguous() else a.clone()
-    if not b.is_contiguous() or b.data_ptr() % 16:
-        raise ValueError("b must be contiguous and 16-byte aligned")
-    return a, a_scale.contiguous(), b, b_scale.contiguous(), _out_rows(out, (m, n), out_dtype, "out", a.device)
+    return _calls().swiglu_quantize(x, dtype, *(out or (None, None)))
 
 
 def mm_8bit(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, out: torch.Tensor | None = None,
             out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
     """out[M, N] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k]: activations in 8 bits with one fp32 scale per token (as `rmsnorm_quantize` and
     `swiglu_quantize` leave them) times weights [N, K] in 8 bits with one per output channel, both int8 (sums exact in int32) or both
-    float8_e4m3fn (sums in fp32). K % 16 == 0, K <= 131071; any M and N. out: bf16, fp16 or fp32 (``out_dtype``, which a given ``out`` must have)."""
-    if out is not None:
-        out_dtype = out.dtype
-    a, a_scale, b, b_scale, out = _mm_8bit_args(a, a_scale, b, b_scale, (), out, out_dtype, status)
-    _lib.check(_lib.load().b200moe_gemm_8bit(a.data_ptr(), _row_stride(a), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), out.data_ptr(),
-                                             a.shape[0], b.shape[0], a.shape[1], _row_stride(out), _CODE_TYPES[a.dtype], _ROW_TYPES[out_dtype],
-                                             _ptr(status), _stream()), "b200moe_gemm_8bit")
-    return out
+    float8_e4m3fn (sums in fp32). K % 16 == 0, K <= 131071; any M and N. out: bf16, fp16 or fp32 (``out_dtype``, or what a given ``out`` has).
+    An int8 row gives the same bits in every batch; an e4m3 row's sums are ordered by the form that its batch takes."""
+    return _calls().mm_8bit(a, a_scale, b, b_scale, None, out, out_dtype, status)
 
 
 def mm_8bit_grouped(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, offsets: torch.Tensor,
                     out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16, status: torch.Tensor | None = None) -> torch.Tensor:
     """`mm_8bit` over the experts' segments of sorted rows: rows offsets[e] .. offsets[e + 1] - 1 times b[e]. offsets int32 [E + 1] on the device
     (`route_sort` makes it); b [E, N, K], b_scale [E, N], E <= 1024. Rows of no segment are zero in a new output and left as they are in a given one."""
-    if out is not None:
-        out_dtype = out.dtype
-    if b.dim() != 3 or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != b.shape[0] + 1:
-        raise ValueError("b must be [E, N, K] and offsets int32 [E + 1]")
-    fresh = out is None
-    a, a_scale, b, b_scale, out = _mm_8bit_args(a, a_scale, b, b_scale, (b.shape[0],), out, out_dtype, status, offsets)
-    offsets = offsets.contiguous()
-    _lib.check(_lib.load().b200moe_gemm_8bit_grouped(a.data_ptr(), _row_stride(a), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
-                                                     offsets.data_ptr(), b.shape[0], out.data_ptr(), a.shape[0], b.shape[1], a.shape[1],
-                                                     _row_stride(out), _CODE_TYPES[a.dtype], _ROW_TYPES[out_dtype], int(fresh), _ptr(status),
-                                                     _stream()), "b200moe_gemm_8bit_grouped")
-    return out
+    return _calls().mm_8bit(a, a_scale, b, b_scale, offsets, out, out_dtype, status)
 
 
 def combine(rows: torch.Tensor, row_of: torch.Tensor, weight_of_row: torch.Tensor, out: torch.Tensor) -> torch.Tensor:

@@ -206,6 +206,55 @@ def test_captured_training_step():
     assert alive.shape == (t, h)
 
 
+def test_capture_beside_a_live_graph_is_refused():
+    """A captured backward pass of leaves whose eager graph lives would end the process: the forward call says so instead."""
+    t, k, e, h = 20, 2, 4, 64
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w = rand((t, h), torch.bfloat16, 1).requires_grad_(), rand((t, k), torch.float32, 2).requires_grad_()
+    alive = ks.unsort_tokens(ks.sort_tokens(x, order), order, w)
+    rows = rand((t * k, h), torch.bfloat16, 3)
+    said = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows.mul_(1.0)
+        for call in (lambda: ks.sort_tokens(x, order), lambda: ks.unsort_tokens(rows, order, w)):
+            try:
+                call()
+            except ValueError as exc:
+                said.append(str(exc))
+    assert len(said) == 2 and all("alive" in s for s in said)
+    assert alive.shape == (t, h)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):                                  # the graph is gone, and its nodes with it
+        y = ks.unsort_tokens(ks.sort_tokens(x, order), order, w).detach()
+    graph.replay()
+    with torch.no_grad():
+        assert torch.equal(y, ks.unsort_tokens(ks.sort_tokens(x, order), order, w))
+
+
+def test_gradients_of_gradients_are_refused():
+    t, k, e, h = 6, 2, 4, 16
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w = rand((t, h), torch.float32, 1).requires_grad_(), rand((t, k), torch.float32, 2).requires_grad_()
+    y = ks.unsort_tokens(ks.sort_tokens(x, order), order, w)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w), create_graph=True)
+    for d in (dx, dw):
+        with pytest.raises(RuntimeError):
+            d.sum().backward(retain_graph=True)
+
+
+def test_backward_accumulates():
+    """.backward() twice, of a scale column as well: gradients add up in .grad."""
+    t, k, e = 40, 3, 8
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    s, m = rand((t,), torch.float32, 1).requires_grad_(), rand((t * k,), torch.float32, 2)
+    for _ in range(2):
+        (ks.sort_tokens(s, order) * m).sum().backward()
+    exact, size = unsort_exact(m[:, None], order, None)
+    close(s.grad, 2 * exact[:, 0], 2 * size[:, 0], 2 * k)
+
+
 def test_empty_batch():
     order = ks.route_sort(torch.empty(0, 4, dtype=torch.int32, device="cuda"), 8)
     assert order.offsets.tolist() == [0] * 9
