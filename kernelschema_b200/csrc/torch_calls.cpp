@@ -176,11 +176,11 @@ std::tuple<Tensor, Tensor, Tensor> route_sort(const Tensor& ids_in, int64_t num_
   const int64_t t = ids.size(0), k = ids.size(1), n = t * k;
   const int64_t need = b200moe_route_sort_workspace_bytes(t, (int32_t)k, (int32_t)num_experts);
   if (need < 0) refuse(std::string("route_sort: ") + b200moe_last_error());
-  const Tensor offsets = fresh({num_experts + 1}, at::kInt, ids), row_of = fresh({t, k}, at::kInt, ids), route_of_row = fresh({n}, at::kInt, ids);
-  Maybe workspace;
-  if (need) workspace = fresh({need}, at::kByte, ids);
+  const Tensor offsets = fresh({num_experts + 1}, at::kInt, ids), row_of = fresh({t, k}, at::kInt, ids);
+  // The workspace lies behind route_of_row: a graph that was not captured by torch has no pool that would keep a buffer of this call alone.
+  const Tensor last = fresh({n + need / 4}, at::kInt, ids), route_of_row = need ? last.narrow(0, 0, n) : last;
   check(b200moe_route_sort(ptr<int32_t>(ids), row_stride(ids), t, (int32_t)k, (int32_t)num_experts, ptr<int32_t>(offsets), ptr<int32_t>(row_of),
-                           ptr<int32_t>(route_of_row), ptr(workspace), need, here.stream()),
+                           ptr<int32_t>(route_of_row), need ? ptr<int32_t>(last) + n : nullptr, need, here.stream()),
         "b200moe_route_sort");
   return {offsets, row_of, route_of_row};
 }

@@ -1,8 +1,13 @@
 """Arguments that the 8-bit operators refuse, checked before any device work (no GPU needed)."""
+import os
+import re
+
 import pytest
 import torch
 
 import kernelschema_b200 as ks
+
+CSRC = os.path.join(os.path.dirname(os.path.abspath(ks.__file__)), "csrc")
 
 
 @pytest.fixture(scope="module")
@@ -126,3 +131,18 @@ def test_route_order_refusals(lib):
 
     assert grad(c=0) == 787 and grad(g=None) == 788 and grad(valid=None) == 788 and grad(r=None) == 788 and grad(gr=17) == 789 and grad(gw=18) == 789
     assert grad(gr=None, gw=None) == 0 and grad(t=0) == 0
+
+
+def test_cluster_kernels_in_headers_let_nothing_in_early():
+    """The rule for cluster kernels holds for those in headers: released by their end alone, they have no pdl_trigger."""
+    seen = set()
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith(".cuh"):
+            continue
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+        for kernel in re.split(r"\b__global__\b", text)[1:]:
+            body = kernel[:kernel.index("\n}\n")]
+            if "cluster" in body:
+                seen.add(re.search(r"\b(k_\w+)\s*\(", body).group(1))
+                assert "pdl_trigger" not in body, name
+    assert seen == {"k_gemm_8bit_pair", "k_gemm_8bit_split"}
