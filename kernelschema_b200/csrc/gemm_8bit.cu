@@ -60,12 +60,16 @@ k_gemm_8bit(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ To
       bool ok = true;
       while (ok && walk.next(p, tb, it)) {
         const int box = g8_box(it.rows), bytes = 128 * 16 << box;
-        for (int ks = 0; ks < nk; ++ks) {
+        for (int ks = 0; ks < nk; ks += C::KC) {
           if (!mbar_wait(bar_empty + 8 * s, ph)) { if (p.status) atomicCAS(p.status, 0, 141); ok = false; break; }
           const uint32_t full = bar_full + 8 * s;
-          mbar_expect_tx(full, C::kWBytes + bytes);
-          tma_load_2d(s_w + s * C::kWBytes, &tm_w, full, ks * 128, it.wrow0);
-          tma_load_2d(s_x + s * C::kXBytes, &tm_x.m[box], full, ks * 128, (int)it.row0);
+          mbar_expect_tx(full, min(C::KC, nk - ks) * (C::kWStep + bytes));
+#pragma unroll
+          for (int c = 0; c < C::KC; ++c) {
+            if (ks + c >= nk) break;
+            tma_load_2d(s_w + s * C::kWBytes + c * C::kWStep, &tm_w, full, (ks + c) * 128, it.wrow0);
+            tma_load_2d(s_x + s * C::kXBytes + c * C::kXStep, &tm_x.m[box], full, (ks + c) * 128, (int)it.row0);
+          }
           if (++s == C::kStages) { s = 0; ph ^= 1; }
         }
       }
@@ -84,13 +88,18 @@ k_gemm_8bit(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ To
         tc_fence_after();
         const uint32_t acc = tmem + buf * MT;
         const uint32_t idesc = idesc_8bit<kInt>(128, it.rows <= 16 ? 16 : (it.rows + 31) & ~31);
-        for (int ks = 0; ks < nk; ++ks) {
+        for (int ks = 0; ks < nk; ks += C::KC) {
           if (!mbar_wait(bar_full + 8 * s, ph)) { if (p.status) atomicCAS(p.status, 0, 143); ok = false; break; }
           tc_fence_after();
           const uint32_t w_lo = w_lo0 + s * (C::kWBytes >> 4), x_lo = x_lo0 + s * (C::kXBytes >> 4);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mma_8bit<kInt>(acc, ((uint64_t)kHi << 32) | (w_lo + 2 * q), ((uint64_t)kHi << 32) | (x_lo + 2 * q), idesc, (ks | q) ? 1u : 0u);
+          for (int c = 0; c < C::KC; ++c) {
+            if (ks + c >= nk) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mma_8bit<kInt>(acc, ((uint64_t)kHi << 32) | (w_lo + c * (C::kWStep >> 4) + 2 * q), ((uint64_t)kHi << 32) | (x_lo + c * (C::kXStep >> 4) + 2 * q), idesc,
+                             (ks | c | q) ? 1u : 0u);
+          }
           mma_commit(bar_empty + 8 * s);
           if (++s == C::kStages) { s = 0; ph ^= 1; }
         }
@@ -175,10 +184,10 @@ struct G8Plan {
 
 // Dense: the form whose estimate is the least. An estimate is in microseconds of a call among others, linear in what its form is made of: waves of
 // blocks, the k-steps of 128 of a wave (dearer the fuller it is), the bytes of the weights, the sums that a cluster exchanges. Fitted to
-// 4400 shapes (1 to 4096 rows, 128 <= N <= 16384, 256 <= K <= 16384, both types, every form timed); choosing by it costs 1 to 2 % on average
-// against always taking the fastest form, 11 % or less for 90 of 100 shapes. Some of the times behind it (us, int8):
-//   1 x 4096 x 7168      decode 8.4, split 9.2, single 12.0          16 x 16384 x 4096   single 13.7, decode 15.4
-//   64 x 1024 x 8192     split 8.0, single 13.6                      256 x 4096 x 7168   single (64 rows) 13.8, split 17.7, pair (256) 23
+// 12000 shapes (1 to 4096 rows, 128 <= N <= 16384, 256 <= K <= 16384, both types, every form timed); choosing by it costs 1 % on average against
+// always taking the fastest form, 8 % or less for 95 of 100 shapes. Some of the times behind it (us, int8):
+//   1 x 4096 x 7168      decode 8.4, split 9.2, single 10.3          16 x 16384 x 4096   single 13.0, decode 15.4
+//   64 x 1024 x 8192     split 8.0, single 12.6                      256 x 4096 x 7168   single (64 rows) 13.8, split 17.7, pair (256) 23
 //   512 x 4096 x 12288   pair (128) 24.7, single 26.9                8192 x 4096 x 12288 pair (256) 255, pair (128) 304, single 362
 G8Plan dense_plan(const Gemm8Params& p) {
   const int sms = sm_count();
@@ -194,11 +203,11 @@ G8Plan dense_plan(const Gemm8Params& p) {
     const bool deep = items <= sms;
     const int64_t slots = deep ? sms : 2 * sms, w = up(items, slots);
     const double full = (double)items / (double)(w * slots), steps = (double)(w * nk);
-    const double us = mt == 16                ? 2.67 * w + steps * (0.160 + 0.178 * full)
-                      : mt == 64 && deep      ? 3.13 * w + steps * (0.189 + 0.086 * full)
-                      : mt == 64              ? 3.92 + 0.55 * w + steps * (0.177 + 0.276 * full)
-                      : deep                  ? 4.09 * w + steps * (0.240 + 0.075 * full)
-                                              : 3.83 + 1.64 * w + steps * (0.347 + 0.222 * full);
+    const double us = mt == 16           ? 2.82 * w + steps * (0.137 + 0.185 * full)
+                      : mt == 64 && deep ? 3.28 * w + steps * (0.176 + 0.095 * full)
+                      : mt == 64         ? 3.84 + 0.65 * w + steps * (0.170 + 0.275 * full)
+                      : deep             ? 4.15 * w + steps * (0.236 + 0.062 * full)
+                                         : 3.97 + 1.75 * w + steps * (0.233 + 0.357 * full);
     offer(us, {kSingle, mt, 1});
   };
   const auto split = [&](int mt, int by, double wave, double step, double fetch, double exchange) {
@@ -210,31 +219,33 @@ G8Plan dense_plan(const Gemm8Params& p) {
           {kSplit, mt, by});
   };
   if (m <= 16 || (m <= 32 && p.code == kInt8)) {
-    const int64_t blocks = up(n, 16), warps = blocks < 222 ? 16 : blocks < 444 ? 8 : 4;
-    const double mb = (double)n * p.K * 1e-6, units = (double)p.K / 64 / (double)warps;
-    offer(m > 16 ? 3.17 + 0.182 * mb + 0.313 * units : p.code == kInt8 ? 2.16 + 0.133 * mb + 0.239 * units : 2.50 + 0.149 * mb + 0.306 * units, {kDecode, 0, 1});
+    // batches of loads of a warp, dearer with the rows; the weights; the blocks
+    const int64_t blocks = up(n, 16);
+    const double batches = (double)up(up(up(p.K, 64), gemm_8bit_decode_warps(blocks, p.K, sms)), 4), mb = (double)n * p.K * 1e-6, kb = (double)blocks * 1e-3;
+    const double r = (double)m / 16;
+    offer(m > 16             ? 2.02 + batches * (0.524 + 0.405 * r) + 0.126 * mb + 2.41 * kb
+          : p.code == kInt8  ? 1.31 + batches * (0.477 + 0.504 * r) + 0.156 * mb + 1.07 * kb
+                             : 1.37 + batches * (0.637 + 0.413 * r) + 0.172 * mb + 0.99 * kb,
+          {kDecode, 0, 1});
   }
   if (m <= 16) {
     single(16);
-    split(16, 4, 4.40, 0.153, 0.0906, 4.62);
-    split(16, 8, 4.48, 0.143, 0.0968, 2.85);
+    split(16, 4, 4.40, 0.160, 0.0921, 4.09);
+    split(16, 8, 4.52, 0.141, 0.1004, 2.51);
     return best;
   }
   if (m <= 640) {
     single(64);
-    split(64, 4, 5.59, 0.207, 0.0393, 1.43);
-    split(64, 8, 5.02, 0.227, 0.0359, 1.40);
+    split(64, 4, 5.53, 0.247, 0.0294, 1.51);
+    split(64, 8, 5.09, 0.209, 0.0509, 1.15);
   }
   if (m > 64) {
     single(128);
-    if (m <= 1500) {
-      split(128, 4, 8.18, 0.242, 0.0392, 0.64);
-      split(128, 8, 6.29, 0.272, 0.0433, 0.81);
-    }
+    if (m <= 1500) split(128, 8, 6.24, 0.280, 0.0360, 0.84);
     for (int mt = 128; mt <= (m > 128 ? 256 : 128); mt *= 2) {
       const int64_t items = up(m, mt) * up(n, 256), pairs = sms / 2, w = up(items, pairs);
       const double full = (double)items / (double)(w * pairs), steps = (double)(w * nk);
-      offer(mt == 128 ? 3.68 + 1.93 * w + steps * (0.192 + 0.034 * full) : 4.32 + 2.74 * w + steps * (0.288 + 0.060 * full), {kPair, mt, 1});
+      offer(mt == 128 ? 3.65 + 1.99 * w + steps * (0.187 + 0.034 * full) : 4.22 + 2.82 * w + steps * (0.287 + 0.057 * full), {kPair, mt, 1});
     }
   }
   return best;

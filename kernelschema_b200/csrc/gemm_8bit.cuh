@@ -16,11 +16,17 @@ constexpr int kG8Group = 8;                                  // token tiles of a
 
 __host__ __device__ constexpr int g8_table_bytes(int experts) { return experts ? 4 * (3 * experts + 2) : 0; }
 
-// MT = most tokens of a tile. Up to 128 two blocks share an SM (half of its shared memory and TMEM each).
+// MT = most tokens of a tile. kDeep: one block has an SM's shared memory, otherwise two share it (and its TMEM).
+// A stage holds KC steps of 128 bytes of K. A step of few tokens takes the tensor core 128 cycles (its 16 KB of weights at 128 bytes a cycle), and
+// the MMA thread's wait and commit about as many: two steps per stage where a long loop of them is the time (16 x 4096 x 7168 12.4 -> 10.3 us,
+// 64 rows 13.1 -> 12.0; four steps leave too few stages: 13.0, 14.4; 128 rows, three stages, 14.8 -> 15.7; narrower tiles of 32 or 64
+// weight rows, which read less per step, take the same time).
 template <int MT, bool kDeep = false>
 struct G8Cfg {
-  static constexpr int kWBytes = 128 * 128, kXBytes = MT * 128, kStageBytes = kWBytes + kXBytes;
-  static constexpr int kStages = kDeep ? (MT == 16 ? 11 : MT == 64 ? 8 : 6) : (MT == 16 ? 5 : MT == 64 ? 4 : 3);
+  static constexpr int KC = kDeep && MT <= 64 ? 2 : 1;
+  static constexpr int kWStep = 128 * 128, kXStep = MT * 128;
+  static constexpr int kWBytes = KC * kWStep, kXBytes = KC * kXStep, kStageBytes = kWBytes + kXBytes;
+  static constexpr int kStages = kDeep ? (MT == 16 ? 5 : MT == 64 ? 4 : 6) : (MT == 16 ? 5 : MT == 64 ? 4 : 3);
   static constexpr int kTmemCols = 2 * MT;
   static constexpr int kBlocksPerSm = kDeep ? 1 : 2;
   static constexpr int kBarBytes = 256;

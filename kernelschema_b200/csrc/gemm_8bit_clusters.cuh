@@ -164,8 +164,8 @@ template <int MT, bool kDeep>
 struct G8Split {
   static constexpr int kStages = kDeep ? (MT == 16 ? 11 : MT == 64 ? 8 : 6) : (MT == 16 ? 6 : MT == 64 ? 4 : 3);
   static constexpr int kTmemCols = MT < 32 ? 32 : MT;
-  static constexpr int kSmem = kStages * G8Cfg<MT>::kStageBytes + 1024 + G8Cfg<MT>::kBarBytes;
-  static_assert(MT * 128 * 4 <= kStages * G8Cfg<MT>::kStageBytes && kSmem <= 232448 && 16 * kStages + 12 <= G8Cfg<MT>::kBarBytes, "the tile's sums take the stages' place");
+  static constexpr int kSmem = kStages * (16384 + MT * 128) + 1024 + G8Cfg<MT>::kBarBytes;
+  static_assert(MT * 128 * 4 <= kStages * (16384 + MT * 128) && kSmem <= 232448 && 16 * kStages + 12 <= G8Cfg<MT>::kBarBytes, "the tile's sums take the stages' place");
 };
 
 template <bool kInt, int MT, bool kDeep>

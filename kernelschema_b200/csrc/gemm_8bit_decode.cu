@@ -121,10 +121,8 @@ __global__ void __launch_bounds__(512) k_gemm_8bit_decode(const uint8_t* __restr
 
 template <bool kInt, int NT>
 int launch_nt(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st) {
-  // warps of a block: enough of them that the device has its bytes in flight, while each has K to work on
-  const int64_t blocks = ((int64_t)p.N + kD8Rows - 1) / kD8Rows, units = (p.K + kD8Unit - 1) / kD8Unit;
-  int warps = 4;
-  while (warps < 16 && blocks * warps < 12ll * sm_count() && warps * 2 <= units) warps *= 2;
+  const int64_t blocks = ((int64_t)p.N + kD8Rows - 1) / kD8Rows;
+  const int warps = gemm_8bit_decode_warps(blocks, p.K, sm_count());
   const int smem = warps * 8 * NT * kD8Rows * 4;
   static SmemOptIn opt_in;
   if (int e = opt_in.ensure(k_gemm_8bit_decode<kInt, NT>, 16 * 8 * NT * kD8Rows * 4)) return e;

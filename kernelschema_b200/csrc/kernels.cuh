@@ -242,7 +242,16 @@ struct Gemm8Params {
   int code, out_type;                        // kInt8 / kE4m3; kBf16 / kF16 / kF32
   int zero_rest;                             // grouped: rows of no segment become zero
 };
-// Few tokens (gemm_8bit_decode.cu).
+// Few tokens (gemm_8bit_decode.cu). Warps of a block, which share its K in units of 64 bytes: as many as the device holds at once (16 per SM,
+// by registers: 11 x 2596 x 4944 in 163 blocks of 16 warps, two waves, 8.9 us), while each has a batch of four units to load (2 x 3033 x 992
+// with 16 warps of one unit 6.1 us).
+inline int gemm_8bit_decode_warps(int64_t blocks, int64_t k, int sms) {
+  const int64_t units = (k + 63) / 64;
+  int warps = 16;
+  while (warps > 2 && blocks * warps > 16ll * sms) warps /= 2;
+  while (warps > 1 && warps * 4 > units) warps /= 2;
+  return warps;
+}
 int launch_gemm_8bit_decode(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
 int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8Params& p, cudaStream_t st);
 

@@ -47,7 +47,8 @@ SHAPES = [(1, 128, 128), (1, 1, 16), (2, 129, 48), (15, 31, 112), (16, 127, 128)
 # one at least for each form that the library chooses among: few and many tiles of 16, 64 and 128 tokens, K split over 4 and 8 blocks, CTA pairs
 SHAPES += [(1, 18470, 128), (9, 23005, 96), (16, 50, 14016), (5, 1223, 10112), (2, 4480, 3568), (17, 19156, 16), (22, 17, 1552), (627, 1, 2304), (17, 5243, 2896),
            (655, 1, 16), (666, 3164, 16), (651, 130, 1776), (1233, 20, 1968), (1339, 260, 5632), (1642, 1, 4288), (1642, 300, 4288), (897, 2509, 1344),
-           (2500, 2700, 1040), (19053, 1, 16), (4097, 600, 2064)]
+           (2500, 2700, 1040), (19053, 1, 16), (4097, 600, 2064), (16, 1, 25328), (3, 3070, 6800), (2, 4746, 3488), (25, 4244, 2992), (609, 1, 2528),
+           (13, 1, 272), (9, 19119, 16), (32, 700, 1488), (12, 40, 192), (5, 33, 64)]
 
 
 @pytest.mark.parametrize("kind", CODES)
