@@ -289,7 +289,12 @@ int launch_gemm_8bit(const void* a, int64_t a_stride, const void* b, const Gemm8
   CUtensorMap tw;
   TokenMaps tx;
   int rc = make_operand_map(&tw, b, (uint64_t)(p.experts ? p.experts : 1) * (uint64_t)p.N, (uint64_t)p.K, 128);
-  for (int i = 0; i < 4 && !rc; ++i) rc = make_operand_map(&tx.m[i], a, (uint64_t)p.M, (uint64_t)p.K, 16u << i, (uint64_t)a_stride);
+  // of the token maps those that a tile of the call can ask for: dense tiles are full but for the last (a map takes 0.2 us to make)
+  const auto box = [&](int64_t rows) { return g8_box((int)(plan.form == kPair ? (rows + 31) / 32 * 16 : rows)); };
+  const int64_t rest = p.M % plan.mt;
+  const unsigned need = p.experts ? 15u : (p.M >= plan.mt ? 1u << box(plan.mt) : 0u) | (rest ? 1u << box(rest) : 0u);
+  for (int i = 0; i < 4 && !rc; ++i)
+    if (need >> i & 1) rc = make_operand_map(&tx.m[i], a, (uint64_t)p.M, (uint64_t)p.K, 16u << i, (uint64_t)a_stride);
   if (rc) return rc;
   return p.code == kInt8 ? launch_plan<true>(tw, tx, p, plan, st) : launch_plan<false>(tw, tx, p, plan, st);
 }

@@ -169,7 +169,7 @@ struct G8Walk {
 struct TokenMaps {
   CUtensorMap m[4];
 };
-DEV int g8_box(int rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3; }
+__host__ DEV int g8_box(int rows) { return rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3; }
 
 // Fills the tables, by the whole block; the caller synchronises.
 template <int MT>

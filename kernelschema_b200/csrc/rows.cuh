@@ -64,8 +64,8 @@ struct Any16 {
     const uint32_t sh = (uint32_t)(uintptr_t)p & 15u;
     a = b = make_uint4(0u, 0u, 0u, 0u);
     if (wanted && whole(p, s)) {
-      a = __ldg(reinterpret_cast<const uint4*>(p - sh));
-      b = __ldg(reinterpret_cast<const uint4*>(p - sh + (sh ? 16 : 0)));
+      a = *reinterpret_cast<const uint4*>(p - sh);           // plain loads: a neighbour's bytes may be written meanwhile (rows in place)
+      b = *reinterpret_cast<const uint4*>(p - sh + (sh ? 16 : 0));
     }
   }
   DEV uint4 take(const uint8_t* p, const Span& s) const {
@@ -77,9 +77,9 @@ struct Any16 {
       const uint8_t* q = p + i * sizeof(T);
       uint32_t v = 0;
       if (q >= s.lo && q + sizeof(T) <= s.hi) {
-        if constexpr (sizeof(T) == 4) v = __ldg(reinterpret_cast<const uint32_t*>(q));
-        else if constexpr (sizeof(T) == 2) v = __ldg(reinterpret_cast<const unsigned short*>(q));
-        else v = __ldg(q);
+        if constexpr (sizeof(T) == 4) v = *reinterpret_cast<const uint32_t*>(q);
+        else if constexpr (sizeof(T) == 2) v = *reinterpret_cast<const unsigned short*>(q);
+        else v = *q;
       }
       const int word = i * (int)sizeof(T) / 4;
       v <<= i * sizeof(T) % 4 * 8;

@@ -190,3 +190,17 @@ def test_empty_and_captured():
     for a, b in zip(got[:3], ks.rmsnorm_quantize(x2, w, r)[:3]):
         assert torch.equal(a, b)
     assert torch.equal(again[0], ks.swiglu_quantize(got[2])[0])
+
+
+@pytest.mark.parametrize("h", (24575, 24576, 24577, 31999))
+def test_norm_of_wide_fp32_rows_off_vectors(h):
+    """Rows whose two outputs share a place in shared memory, and the widest that have two; every output beside guard columns."""
+    x, r, w = rows(3, h, torch.float32, 1, pad=3), rows(3, h, torch.float32, 2, pad=3), 1 + 0.1 * rows(1, h, torch.float32, 3)[0]
+    he, y = norm_exact(x, w, r, 1e-6)
+    wide = [torch.full((3, h + 3), -17, dtype=d, device="cuda") for d in (torch.int8, torch.float32, torch.float32)]
+    q, s, hidden, n = ks.rmsnorm_quantize(x, w, r, out=(wide[0][:, 1:h + 1], None, wide[1][:, 2:h + 2], wide[2][:, 3:]))
+    check_codes(q, s, y, torch.int8)
+    assert torch.equal(hidden, x + r)
+    assert bool(((n.double() - y).abs() <= 2 * REL * y.abs() + 1e-38).all())
+    for b, first in zip(wide, (1, 2, 3)):
+        assert bool((b[:, :first] == -17).all()) and bool((b[:, first + h:] == -17).all())
