@@ -5,8 +5,12 @@
 // or 32: a tile of few tokens is no padding, and an expert's rest of rows costs what it holds. A thread of the epilogue then owns an
 // output channel (one sb in a register) and a warp writes 32 consecutive channels of a token, so odd widths, strides and addresses
 // need no form of their own.
-// kind::i8 and kind::f8f6f4 take 32 bytes of K per instruction: a stage of 128 bytes of K is four of them, 64-byte-per-cycle operand
-// reads as for any type. K beyond the last 128-byte step reads as zeros (TMA's fill), so K needs no more than 16-byte rows.
+// kind::i8 and kind::f8f6f4 take 32 bytes of K per instruction, four per step of 128 bytes. K beyond the last step reads as zeros (TMA's fill), so
+// rows need no more than 16-byte lengths.
+//
+// What bounds it: many tokens, the tensor cores (8192 x 4096 x 12288 int8 256 us = 3.2 P op/s, 96 % busy; sustained, the power cap); few, the weight
+// stream (64 tokens over 128 experts 305 MB in 53 us = 5.9 TB/s) and, below about 20 MB of weights, launch, first access and
+// reduction (100 x 2113 x 7168 10.7 us). The forms and their times are at dense_plan.
 #include "gemm_8bit.cuh"
 #include "gemm_8bit_clusters.cuh"
 

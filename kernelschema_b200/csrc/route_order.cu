@@ -8,6 +8,8 @@
 //   gradient   drows[row_of[t, k]] = w[t, k] * dy[t], zeros behind offsets[E];  dw[t, k] = <rows[row_of[t, k]], dy[t]>
 //
 // No atomics on global memory, every sum in a fixed order: the same inputs give the same bits.
+// The row kernels are bound by HBM (8192 x 8 routes, 2048 wide bf16: sort 51 us = 5.9 TB/s, mostly writes; unsort 51 = 6.0; gradient 102 = 5.6), the
+// order by the latency of its one or two launches (64 routes 3 us, 65536 10).
 #include "kernels.cuh"
 #include "rows.cuh"
 

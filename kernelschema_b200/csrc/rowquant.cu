@@ -4,7 +4,7 @@
 //   both       amax = max|y|,  scale = amax / Q,  q = round_to_nearest_even(y * (Q / amax)),  Q = 127 (int8) or 448 (e4m3)
 //
 // Both are bound by HBM: every input element is read once, every output element written once, and a row stays in registers between its
-// reductions. h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
+// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 48 us = 5.3, 16384 x 2048 27.8 = 6.0). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
 // from the fp32 value (the norm sees h before it is rounded to the stream's type).
 // A row holds no scale when it has no finite amax: a NaN or an infinity in it, or a sum of squares beyond fp32, makes the scale NaN and
 // the codes zero, so that the row is NaN wherever it is multiplied out. A row whose amax is below 2^-116 counts as zero (scale 0,
@@ -12,6 +12,8 @@
 //
 // Rows that vectors do not fit (odd widths, strides or addresses) are read as vectors shifted into place (Any16), so a thread holds the
 // same columns as otherwise, and written through shared memory, from where they go out in aligned vectors with single elements at the two ends.
+// They are bound by instructions (8192 x 4099 83 us where 4096 columns take 40). A block that keeps its weights for several rows (88), one barrier for
+// three outputs in places of their own (83) gave nothing; element by element it is 140.
 #include "kernels.cuh"
 #include "rows.cuh"
 
