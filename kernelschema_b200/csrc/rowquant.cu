@@ -4,7 +4,7 @@
 //   both       amax = max|y|,  scale = amax / Q,  q = round_to_nearest_even(y * (Q / amax)),  Q = 127 (int8) or 448 (e4m3)
 //
 // Both are bound by HBM: every input element is read once, every output element written once, and a row stays in registers between its
-// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 48 us = 5.3, 16384 x 2048 27.8 = 6.0). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
+// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 45 us = 5.6, 16384 x 2048 27.8 = 6.0). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
 // from the fp32 value (the norm sees h before it is rounded to the stream's type).
 // A row holds no scale when it has no finite amax: a NaN or an infinity in it, or a sum of squares beyond fp32, makes the scale NaN and
 // the codes zero, so that the row is NaN wherever it is multiplied out. A row whose amax is below 2^-116 counts as zero (scale 0,
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(row_threads<T, VPT, kWarp>()) k_rmsnorm_quanti
   const T* r = p.residual ? (const T*)p.residual + at.row * p.residual_stride : nullptr;
   const Span sx = span_of<T>(p.x, p.rows, p.x_stride, p.cols, x), sr = span_of<T>(p.residual, p.rows, p.residual_stride, p.cols, r);
   const T* rows_r = r ? r : x;                               // any address: nothing is fetched without a residual
-  Fetch16<T, kAny> xf[VPT], rf[VPT];
+  Fetch16<T, kAny, !kWarp> xf[VPT], rf[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = at.v0 + i * at.step;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(row_threads<T, VPT, kWarp>()) k_swiglu_quantiz
   const bool live = at.r < rows;
   const T* g = (const T*)p.x + at.row * p.x_stride;
   const Span sx = span_of<T>(p.x, p.rows, p.x_stride, 2 * (int64_t)p.cols, g);
-  Fetch16<T, kAny> gf[VPT], uf[VPT];
+  Fetch16<T, kAny, !kWarp> gf[VPT], uf[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = at.v0 + i * at.step;
