@@ -734,7 +734,7 @@ int b200moe_gemm_8bit_grouped(const void* a, int64_t a_stride, const float* a_sc
 }
 
 static int order_sizes(const char* what, int64_t T, int32_t top_k) {
-  if (T < 0 || top_k <= 0 || T * top_k > INT32_MAX || T > INT32_MAX) return fail(787, "%s: need tokens >= 0, top_k > 0 and fewer than 2^31 routes", what);
+  if (T < 0 || top_k <= 0 || T > INT32_MAX || T * top_k > INT32_MAX) return fail(787, "%s: need tokens >= 0, top_k > 0 and fewer than 2^31 routes", what);
   return 0;
 }
 

@@ -8,8 +8,10 @@
 //   gradient   drows[row_of[t, k]] = w[t, k] * dy[t], zeros behind offsets[E];  dw[t, k] = <rows[row_of[t, k]], dy[t]>
 //
 // No atomics on global memory, every sum in a fixed order: the same inputs give the same bits.
-// The row kernels are bound by HBM (8192 x 8 routes, 2048 wide bf16: sort 51 us = 5.9 TB/s, mostly writes; unsort 51 = 6.0; gradient 102 = 5.6), the
+// The row kernels are bound by HBM (8192 x 8 routes, 2048 wide bf16: sort 50 us = 6.0 TB/s, mostly writes; unsort 50 = 6.0; gradient 102 = 5.6), the
 // order by the latency of its one or two launches (64 routes 3 us, 65536 10).
+#include <algorithm>
+
 #include "kernels.cuh"
 #include "rows.cuh"
 
@@ -265,17 +267,19 @@ __global__ void __launch_bounds__(kRowThreads) k_sort_rows(const uint8_t* __rest
     const uint8_t* from = x + t * x_stride;
     const int lane = (int)sp.lane, all = (int)sp.lanes;
     if constexpr (!kAny) {
-      uint4 v[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if ((lane + j * all) * 16 < row_bytes) v[j] = __ldg(reinterpret_cast<const uint4*>(from) + lane + j * all);
-      for (int k = 0; k < K; ++k) {
-        const int row = __ldg(row_of + t * K + k);
-        if ((uint32_t)row >= (uint64_t)n_rows) continue;
-        uint4* dst = reinterpret_cast<uint4*>(rows + (int64_t)row * row_bytes);
+      for (int i = lane; i * 16 < row_bytes; i += N * all) {
+        uint4 v[N];
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if ((lane + j * all) * 16 < row_bytes) dst[lane + j * all] = v[j];
+          if ((i + j * all) * 16 < row_bytes) v[j] = __ldg(reinterpret_cast<const uint4*>(from) + i + j * all);
+        for (int k = 0; k < K; ++k) {
+          const int row = __ldg(row_of + t * K + k);
+          if ((uint32_t)row >= (uint64_t)n_rows) continue;
+          uint4* dst = reinterpret_cast<uint4*>(rows + (int64_t)row * row_bytes);
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if ((i + j * all) * 16 < row_bytes) dst[i + j * all] = v[j];
+        }
       }
     } else {
       const Span sx{x, x + (T - 1) * x_stride + row_bytes, from - 15 >= x && from + row_bytes + 32 <= x + (T - 1) * x_stride + row_bytes};
@@ -536,9 +540,10 @@ __global__ void __launch_bounds__(kRowThreads) k_unsort_backward(const UnsortPar
 
 unsigned blocks_of(int64_t n, int64_t per) { return (unsigned)((n + per - 1) / per); }
 
-// `threads` for each of T tokens, fewer where the grid's threads would pass 2^31 (a thread then takes more pieces).
+// `threads` for each of T tokens, fewer where the grid's threads would pass 2^31 (a thread then takes more pieces), but not below the 32 that
+// write a row's ends: 32 for each of 2^26 - 1 tokens still fit.
 Spread spread(int64_t threads, int64_t T) {
-  while (threads > 32 && threads * T > INT32_MAX - kRowThreads) threads = (threads + 1) / 2;
+  while (threads > 32 && threads * T > INT32_MAX - kRowThreads) threads = std::max<int64_t>(32, (threads + 1) / 2);
   Spread s{};
   s.lanes = (uint32_t)threads;
   while ((1ull << s.shift) < (uint64_t)threads) ++s.shift;

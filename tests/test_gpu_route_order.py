@@ -267,6 +267,18 @@ def test_empty_batch():
     assert dx.shape == x.shape and dw.shape == w.shape
 
 
+@pytest.mark.parametrize("t,h", [(1 << 16, 265), (66_000_000, 265)])
+def test_unsort_of_one_row_for_all(t, h):
+    """A row that every token has; 66 million of 33 vectors and an element are more than a grid's threads (35 GB of output)."""
+    if t * h * 2.4 > torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved() - torch.cuda.memory_allocated():
+        pytest.skip("not enough device memory")
+    x = torch.randint(-127, 128, (1, h), device="cuda").to(torch.bfloat16)
+    order = ks.route_sort(torch.zeros(t, 1, device="cuda", dtype=torch.int32), 1)
+    y = ks.unsort_tokens(x.expand(t, -1), order)
+    for part in y.split(1 << 20):
+        assert bool((part == x).all())
+
+
 def test_rows_behind_2_31_elements():
     """2^21 rows of 1032: element offsets pass 2^31."""
     t, k, e, h = 1 << 19, 4, 8, 1032
