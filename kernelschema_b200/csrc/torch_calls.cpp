@@ -14,6 +14,8 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/b200moe.h"
 
@@ -250,16 +252,28 @@ std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Tenso
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+bool is_captured(const c10::Stream& stream) {
+  const cudaStream_t handle = c10::cuda::CUDAStream(stream).stream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  return handle && cudaStreamIsCapturing(handle, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+}
+
 // A graph that was built outside a capture and is still alive keeps the gradient node of its leaf on the stream it was built on; a backward pass
 // that is captured would have to wait for that stream, which ends the process inside autograd's worker thread. So the call is refused while
-// it can be.
+// it can be: where a node that t's gradient will reach, its leaves' among them, is on a stream that is not captured.
 void check_capture(const Tensor& t) {
-  if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf() || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return;
-  const auto stream = node->stream();
-  if (stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap())
-    refuse("a graph of this leaf from outside the capture is still alive: let it go, or capture with x.detach().requires_grad_()");
+  if (!t.is_cuda() || !t.requires_grad() || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> open{t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!open.empty()) {
+    const auto node = open.back();
+    open.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    const auto stream = node->stream();
+    if (stream && *stream != c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap() && !is_captured(*stream))
+      refuse("a graph of this leaf from outside the capture is still alive: let it go, or capture with x.detach().requires_grad_()");
+    for (const auto& edge : node->next_edges()) open.push_back(edge.function);
+  }
 }
 
 // Gradients that have none themselves, as torch's once_differentiable makes them.

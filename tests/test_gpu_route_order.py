@@ -233,6 +233,42 @@ def test_capture_beside_a_live_graph_is_refused():
         assert torch.equal(y, ks.unsort_tokens(ks.sort_tokens(x, order), order, w))
 
 
+def test_capture_beside_a_live_graph_of_an_input_is_refused():
+    """The same where the leaf is behind an operation of the capture, or the whole input was made outside it."""
+    t, k, e, h = 20, 2, 4, 64
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w = rand((t, h), torch.bfloat16, 1).requires_grad_(), rand((t, k), torch.float32, 2).requires_grad_()
+    rows = rand((t * k, h), torch.bfloat16, 3)
+    alive = x * 2
+    said = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: ks.sort_tokens(x + 1, order), lambda: ks.sort_tokens(alive, order), lambda: ks.unsort_tokens(rows, order, w * w)):
+            try:
+                call()
+            except ValueError as exc:
+                said.append(str(exc))
+    assert len(said) == 2 and all("alive" in s for s in said)      # w has no graph outside
+
+
+def test_capture_on_two_streams():
+    """A stream that joined the capture is part of it: its nodes refuse nothing, and the gradients are those of eager calls."""
+    t, k, e, h = 20, 2, 4, 64
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, g = rand((t, h), torch.float32, 1).requires_grad_(), rand((t * k, h), torch.float32, 3)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            twice = x * 2
+        torch.cuda.current_stream().wait_stream(side)
+        dx, = torch.autograd.grad(ks.sort_tokens(twice, order), x, g)
+    graph.replay()
+    eager, = torch.autograd.grad(ks.sort_tokens(x * 2, order), x, g)
+    assert torch.equal(dx, eager)
+
+
 def test_gradients_of_gradients_are_refused():
     t, k, e, h = 6, 2, 4, 16
     order = ks.route_sort(make_ids(t, k, e, 1), e)
