@@ -3,6 +3,7 @@
 // and allocations take 12 us in Python and 3 us here. Nothing is computed here and nothing kept between calls.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
@@ -248,6 +249,11 @@ std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Tenso
   return {grad_rows, grad_weights};
 }
 
+// Whether t carries a tangent that forward-mode differentiation asks for. A dual tensor does not require a gradient, and the kernels read its
+// primal part alone.
+bool has_tangent(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
+bool has_tangent(const Maybe& t) { return t && has_tangent(*t); }
+
 // ---- gradients of the token sorting
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -310,7 +316,12 @@ struct UnsortTokens : torch::autograd::Function<UnsortTokens> {
   }
 };
 
+void refuse_tangents(bool any) {
+  if (any) refuse("sort_tokens and unsort_tokens have no forward-mode derivative");
+}
+
 Tensor sort_tokens(const Tensor& x, const Tensor& offsets, const Tensor& row_of) {
+  refuse_tangents(has_tangent(x));
   if (!at::GradMode::is_enabled() || !x.requires_grad()) return sort_rows(x, offsets, row_of);
   if (row_type(x.scalar_type()) < 0) refuse("sort_tokens has a gradient for bf16, fp16 and fp32 rows");
   check_capture(x);
@@ -318,6 +329,7 @@ Tensor sort_tokens(const Tensor& x, const Tensor& offsets, const Tensor& row_of)
 }
 
 Tensor unsort_tokens(const Tensor& rows, const Tensor& offsets, const Tensor& row_of, const Maybe& weights) {
+  refuse_tangents(has_tangent(rows) || has_tangent(weights));
   if (!at::GradMode::is_enabled() || !(rows.requires_grad() || (weights && weights->requires_grad()))) return unsort_rows(rows, offsets, row_of, weights);
   check_capture(rows);
   if (weights) check_capture(*weights);

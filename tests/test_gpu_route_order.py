@@ -328,3 +328,19 @@ def test_rows_behind_2_31_elements():
     wide = rows.to(torch.bfloat16)
     y = ks.unsort_tokens(wide, order, torch.full((t, k), 0.25, device="cuda"))
     assert torch.equal(y, x.to(torch.bfloat16))
+
+
+def test_function_transforms_and_tangents_raise():
+    """What the calls have no rule for is an error, not a derivative of zero."""
+    import torch.autograd.forward_ad as forward_ad
+    t, k, e, h = 12, 2, 4, 32
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w, rows = rand((t, h), torch.float32, 1), rand((t, k), torch.float32, 2), rand((t * k, h), torch.float32, 3)
+    for f, args in ((lambda v: ks.sort_tokens(v, order), (x,)), (lambda v, u: ks.unsort_tokens(v, order, u), (rows, w))):
+        ones = tuple(torch.ones_like(v) for v in args)
+        for transform in (lambda: torch.func.jvp(f, args, ones), lambda: torch.func.grad(lambda *v: f(*v).sum())(*args), lambda: torch.func.vmap(f)(*(v[None] for v in args))):
+            with pytest.raises((RuntimeError, ValueError)):
+                transform()
+        for i in range(len(args)):
+            with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+                f(*(forward_ad.make_dual(v, o) if j == i else v for j, (v, o) in enumerate(zip(args, ones))))

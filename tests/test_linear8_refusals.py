@@ -133,6 +133,24 @@ def test_route_order_refusals(lib):
     assert grad(gr=None, gw=None) == 0 and grad(t=0) == 0
 
 
+def test_tangents_are_refused():
+    """Forward-mode differentiation would lose its tangent (a dual tensor does not require a gradient), so the sorting calls refuse it."""
+    import torch.autograd.forward_ad as forward_ad
+    i32, f = torch.int32, torch.float32
+    order = ks.RouteOrder(z(9, dtype=i32), z(4, 2, dtype=i32), z(8, dtype=i32))
+    with forward_ad.dual_level():
+        dual = lambda v: forward_ad.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (lambda: ks.sort_tokens(dual(z(4, 64)), order), lambda: ks.sort_tokens(dual(z(4, dtype=f)), order), lambda: ks.unsort_tokens(dual(z(8, 64)), order),
+                     lambda: ks.unsort_tokens(z(8, 64), order, dual(z(4, 2, dtype=f))), lambda: ks.unsort_tokens(z(8, 64).requires_grad_(), order, dual(z(4, 2, dtype=f)))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):     # which leaves forward mode on
+                call()
+        x = dual(z(4, 64))
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
+            ks.sort_tokens(x, order)                               # no tangent is asked for: a call like any other
+
+
 def test_cluster_kernels_in_headers_let_nothing_in_early():
     """The rule for cluster kernels holds for those in headers: released by their end alone, they have no pdl_trigger."""
     seen = set()
