@@ -95,6 +95,21 @@ Tensor out_values(const Maybe& out, int64_t n, const char* name, const Tensor& l
   return *out;
 }
 
+bool wants_gradient(const Tensor& t) { return t.requires_grad(); }
+bool wants_gradient(const Maybe& t) { return t && t->requires_grad(); }
+// Whether t carries a tangent that forward-mode differentiation asks for. A dual tensor does not require a gradient, and the kernels read its
+// primal part alone.
+bool has_tangent(const Tensor& t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
+bool has_tangent(const Maybe& t) { return t && has_tangent(*t); }
+
+// The 8-bit operators have no derivative: tensors that ask for one are refused, their results would come without it.
+template <class... Ts>
+void no_derivative(const char* what, const Ts&... ts) {
+  if (at::GradMode::is_enabled() && (wants_gradient(ts) || ...))
+    refuse(std::string(what) + " has no gradient: pass detached tensors, or call it under torch.no_grad()");
+  if ((has_tangent(ts) || ...)) refuse(std::string(what) + " has no forward-mode derivative");
+}
+
 int wanted_codes(ScalarType dtype) {
   const int code = code_type(dtype);
   if (code < 0) refuse("dtype must be torch.int8 or torch.float8_e4m3fn");
@@ -111,6 +126,7 @@ std::tuple<Tensor, Tensor, Tensor, Maybe> rmsnorm_quantize(const Tensor& x_in, c
   if (weight_in.dim() != 1 || weight_in.size(0) != h || (weight_in.scalar_type() != x_in.scalar_type() && weight_in.scalar_type() != at::kFloat))
     refuse("weight must be [" + std::to_string(h) + "] in x's type or float32");
   const int code = wanted_codes(dtype);
+  no_derivative("rmsnorm_quantize", x_in, weight_in, residual_in, q_out, scale_out, hidden_out, norm_out);
   const Here here(x_in, weight_in, residual_in, q_out, scale_out, hidden_out, norm_out);
   const Tensor x = unit_rows(x_in), weight = weight_in.contiguous();
   const Maybe residual = residual_in ? Maybe(unit_rows(*residual_in)) : Maybe();
@@ -128,6 +144,7 @@ std::tuple<Tensor, Tensor> swiglu_quantize(const Tensor& x_in, ScalarType dtype,
   const int rows = row_type(x_in.scalar_type());
   if (x_in.dim() != 2 || rows < 0 || x_in.size(1) % 2 || !x_in.size(1)) refuse("swiglu_quantize expects bf16, fp16 or fp32 [T, 2I]");
   const int code = wanted_codes(dtype);
+  no_derivative("swiglu_quantize", x_in, q_out, scale_out);
   const Here here(x_in, q_out, scale_out);
   const Tensor x = unit_rows(x_in);
   const int64_t t = x.size(0), i = x.size(1) / 2;
@@ -153,6 +170,7 @@ Tensor mm_8bit(const Tensor& a_in, const Tensor& a_scale_in, const Tensor& b, co
   const int out_type = row_type(out_dtype);
   if (out_type < 0) refuse("the output must be bfloat16, float16 or float32");
   if (status && (status->scalar_type() != at::kInt || !status->numel())) refuse("status must be an int32 tensor");
+  no_derivative(lead ? "mm_8bit_grouped" : "mm_8bit", a_in, a_scale_in, b, b_scale_in, out_in);
   const Here here(a_in, a_scale_in, b, b_scale_in, offsets_in, out_in, status);
   Tensor a = unit_rows(a_in);
   if (row_stride(a) < k || row_stride(a) % 16 || (uintptr_t)a.data_ptr() % 16) a = a.clone(at::MemoryFormat::Contiguous);
@@ -248,11 +266,6 @@ std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Tenso
         "b200moe_unsort_rows_backward");
   return {grad_rows, grad_weights};
 }
-
-// Whether t carries a tangent that forward-mode differentiation asks for. A dual tensor does not require a gradient, and the kernels read its
-// primal part alone.
-bool has_tangent(const Tensor& t) { return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
-bool has_tangent(const Maybe& t) { return t && has_tangent(*t); }
 
 // ---- gradients of the token sorting
 using torch::autograd::AutogradContext;

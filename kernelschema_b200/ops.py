@@ -249,7 +249,8 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     fp32. ``hidden`` is h in x's type (x itself without a residual); ``normed`` is y in x's type where asked for, else None. ``out`` = (q,
     scale, hidden, normed): caller-owned buffers, each may be None; hidden may be x or residual themselves (in place).
     h and the sums are fp32, and h is not rounded before the norm. A row of zeros (max|y| < 2^-116) has scale 0; a row with a NaN or an infinity, or whose
-    squares' sum leaves fp32, has scale NaN and codes 0. For inference: this and the other 8-bit operators have no gradient, `hidden` included."""
+    squares' sum leaves fp32, has scale NaN and codes 0. For inference: this and the other 8-bit operators have no gradient, `hidden` included,
+    and refuse tensors that require one while grad mode is on (parameters: call under `torch.no_grad()`)."""
     return _calls().rmsnorm_quantize(x, weight, residual, eps, dtype, normed, *(out or (None, None, None, None)))
 
 

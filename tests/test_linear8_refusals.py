@@ -151,6 +151,33 @@ def test_tangents_are_refused():
             ks.sort_tokens(x, order)                               # no tangent is asked for: a call like any other
 
 
+def test_8bit_operators_refuse_tensors_that_want_a_derivative():
+    """The results of the 8-bit operators hang on no graph: an input that requires a gradient, or has a tangent, is refused instead of losing it."""
+    import torch.autograd.forward_ad as forward_ad
+    i8, f, e4m3 = torch.int8, torch.float32, torch.float8_e4m3fn
+    off = z(2, dtype=torch.int32)
+    grouped = lambda a, sa, b, sb, out=None: ks.mm_8bit_grouped(a, sa, b[None], sb[None], off, out)  # noqa: E731
+    norm = lambda x, w, r, hidden, normed: ks.rmsnorm_quantize(x, w, r, out=(None, None, hidden, normed))  # noqa: E731
+    swiglu = lambda x, s: ks.swiglu_quantize(x, out=(None, s))  # noqa: E731
+    x, w, codes = z(4, 64), z(64), (z(4, 64, dtype=i8), z(32, 64, dtype=i8))
+    for call, args, named in ((norm, (x, w, x, x, x), "rmsnorm_quantize"), (swiglu, (x, z(4, dtype=f)), "swiglu_quantize"),
+                              (ks.mm_8bit, (codes[0], z(4, dtype=f), codes[1], z(32, dtype=f), z(4, 32)), "mm_8bit"),
+                              (grouped, (codes[0], z(4, dtype=f), codes[1], z(32, dtype=f), z(4, 32)), "mm_8bit_grouped"),
+                              (ks.mm_8bit, (z(4, 64, dtype=e4m3), z(4, dtype=f), z(32, 64, dtype=e4m3), z(32, dtype=f)), "mm_8bit")):
+        for i, v in enumerate(args):
+            if not v.is_floating_point():
+                continue
+            wants = args[:i] + (v.clone().requires_grad_(),) + args[i + 1:]
+            with pytest.raises(ValueError, match=named + " has no gradient"):
+                call(*wants)
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):         # nothing is asked for: a call like any other
+                call(*wants)
+            if v.dtype == e4m3:
+                continue
+            with forward_ad.dual_level(), pytest.raises(ValueError, match=named + " has no forward-mode"):
+                call(*args[:i], forward_ad.make_dual(v, torch.ones_like(v)), *args[i + 1:])
+
+
 def test_cluster_kernels_in_headers_let_nothing_in_early():
     """The rule for cluster kernels holds for those in headers: released by their end alone, they have no pdl_trigger."""
     seen = set()
