@@ -4,7 +4,7 @@
 //   both       amax = max|y|,  scale = amax / Q,  q = round_to_nearest_even(y * (Q / amax)),  Q = 127 (int8) or 448 (e4m3)
 //
 // Both are bound by HBM: every input element is read once, every output element written once, and a row stays in registers between its
-// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 45 us = 5.6, 16384 x 2048 27.8 = 6.0). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
+// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 43 us = 5.8, 16384 x 2048 27 = 6.2). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
 // from the fp32 value (the norm sees h before it is rounded to the stream's type).
 // A row holds no scale when it has no finite amax: a NaN or an infinity in it, or a sum of squares beyond fp32, makes the scale NaN and
 // the codes zero, so that the row is NaN wherever it is multiplied out. A row whose amax is below 2^-116 counts as zero (scale 0,
@@ -14,6 +14,8 @@
 // same columns as otherwise, and written through shared memory, from where they go out in aligned vectors with single elements at the two ends.
 // They are bound by instructions (8192 x 4099 83 us where 4096 columns take 40). A block that keeps its weights for several rows (88), one barrier for
 // three outputs in places of their own (83) gave nothing; element by element it is 140.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "rows.cuh"
 
@@ -331,7 +333,37 @@ __global__ void __launch_bounds__(row_threads<T, VPT, kWarp>()) k_rmsnorm_quanti
 }
 
 // ----------------------------------------------------------------------------- SwiGLU
-DEV float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// g * sigmoid(g) * u = g / (1 + exp(-g)) * u, while the quotient is a normal number. (The approximations flush subnormals and meet none.)
+constexpr float kFarGate = -87.f;
+DEV float silu_mul(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));             // log2(e)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r * u;
+}
+// The same for any g: with e = exp(-|g| / 2) sigmoid is 1 / (1 + e^2) above zero and e^2 / (1 + e^2) below, where u comes in between the two e. A large u
+// lifts y above the least amax down to a gate of -174, and so far e is a normal number. Taken for vectors with a gate below kFarGate: for
+// every element it is dearer (65536 x 768 49 us instead of 43).
+DEV float silu_mul_far(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -0.72134752f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, e, 1.f)));
+  const float f = g < 0.f ? e : 1.f;
+  return g * r * (f * u) * f;
+}
+
+// The least element of a vector (a NaN is none).
+DEV float least(const Vec<float>& x) { return fminf(fminf(x.v[0], x.v[1]), fminf(x.v[2], x.v[3])); }
+template <class T>
+DEV float least(const Vec<T>& x) {
+  using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+  union {
+    uint4 raw;
+    T2 pair[4];
+  } p{x.raw};
+  const T2 m = __hmin2(__hmin2(p.pair[0], p.pair[1]), __hmin2(p.pair[2], p.pair[3]));
+  return fminf(to_f32(m.x), to_f32(m.y));
+}
 
 template <class T, int VPT, bool kWarp, bool kAny>
 __global__ void __launch_bounds__(row_threads<T, VPT, kWarp>()) k_swiglu_quantize(const SwigluParams p, const int lanes) {
@@ -367,11 +399,15 @@ __global__ void __launch_bounds__(row_threads<T, VPT, kWarp>()) k_swiglu_quantiz
         cut_vec<T>(uv, v, p.cols);
       }
     }
+    if (!(least(gv) < kFarGate)) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      y[i][j] = silu_mul(to_f32(gv.v[j]), to_f32(uv.v[j]));
-      amax = max(amax, abs_bits(y[i][j]));
+      for (int j = 0; j < E; ++j) y[i][j] = silu_mul(to_f32(gv.v[j]), to_f32(uv.v[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) y[i][j] = silu_mul_far(to_f32(gv.v[j]), to_f32(uv.v[j]));
     }
+#pragma unroll
+    for (int j = 0; j < E; ++j) amax = max(amax, abs_bits(y[i][j]));
   }
   amax = row_max<kWarp>(amax, red_max, lanes);
   store_codes<T, VPT, kWarp, kAny>(p.q, p.q_stride, p.scale, y, amax, p.q_type, at, p.cols, rows, reinterpret_cast<uint8_t*>(row_smem));

@@ -204,3 +204,30 @@ def test_norm_of_wide_fp32_rows_off_vectors(h):
     assert bool(((n.double() - y).abs() <= 2 * REL * y.abs() + 1e-38).all())
     for b, first in zip(wide, (1, 2, 3)):
         assert bool((b[:, :first] == -17).all()) and bool((b[:, first + h:] == -17).all())
+
+
+@pytest.mark.parametrize("kind", ("bf16", "fp32"))
+@pytest.mark.parametrize("i", (64, 1025, 2048))
+def test_swiglu_of_gates_far_below_zero(i, kind):
+    """exp(-gate) leaves fp32 from -88.7 on while `up` may lift the product far above 2^-116: down to a gate of -170 nothing is lost.
+    Tolerance in steps of 2^-23: an exponential of gate / 2 is off by two, and by what the roundings of its argument and of log2(e) move it, |gate| / 2 at most;
+    it counts twice (its square); the reciprocal, the products and the scale add five: 9 + |gate|, and a tenth of that for their products."""
+    pairs = [(-88.0, 1e10), (-87.5, 3e38), (-88.5, -1e5), (-100.0, 3e38), (-126.0, -1e38), (-140.0, 1e38), (-170.0, 3e38), (-60.0, 1e-3), (-1.0, 1e30), (-0.5, -2.0)]
+    x = torch.zeros(len(pairs) + 2, 2 * i, device="cuda")
+    for r, (g, u) in enumerate(pairs):
+        x[r, 5], x[r, i + 5] = g, u
+        x[r, 9], x[r, i + 9] = g, u / 2
+    x[-2, 3], x[-2, i + 3] = -190.0, 3e38                    # 3e-42: below 2^-116
+    x[-1, 3], x[-1, i + 3] = -3e38, 3e38
+    x = x.to(KINDS[kind])
+    g, u = x[:, :i].double(), x[:, i:].double()
+    y = g * torch.sigmoid(g) * u
+    for dtype, top in TOP.items():
+        q, s = ks.swiglu_quantize(x, dtype)
+        for r in range(len(pairs)):
+            exact, steps = float(y[r].abs().max()) / top, (9 + float(g[r].abs().max())) * 1.1
+            assert abs(float(s[r]) - exact) <= exact * steps * 2.0 ** -23, (r, float(s[r]), exact)
+            sign = float(y[r, 5].sign())
+            assert float(q[r, 5].float()) == sign * top and float(q[r, 9].float()) * sign in (64.0, 63.0, 224.0)
+            assert int((q[r].float() != 0).sum()) == 2
+        assert not bool(s[-2:].any()) and not bool(q[-2:].float().any())
