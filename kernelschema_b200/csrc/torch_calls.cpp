@@ -249,20 +249,25 @@ Tensor unsort_rows(const Tensor& rows_in, const Tensor& offsets, const Tensor& r
   return y;
 }
 
-std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Tensor& rows_in, const Tensor& offsets, const Tensor& row_of, const Maybe& weights_in,
-                                              bool want_rows, bool want_weights) {
-  check_rows(rows_in, offsets, row_of, weights_in);
-  if (grad_in.dim() != 2 || grad_in.scalar_type() != rows_in.scalar_type() || grad_in.size(0) != row_of.size(0) || grad_in.size(1) != rows_in.size(1))
-    refuse("the gradient must be like the output of unsort_tokens");
+// The gradient of the rows reads the weights (none: 1), the gradient of the weights the rows: where `rows` is given, it is asked for.
+std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Maybe& rows_in, const Tensor& offsets, const Tensor& row_of, const Maybe& weights_in,
+                                              bool want_rows) {
+  const int type = row_type(grad_in.scalar_type());
+  check_order(offsets, row_of, grad_in.dim() == 2 ? grad_in.size(0) : -1, -1);
+  if (grad_in.dim() != 2 || type < 0) refuse("the gradient must be like the output of unsort_tokens");
+  if (rows_in) {
+    check_rows(*rows_in, offsets, row_of, weights_in);
+    if (grad_in.scalar_type() != rows_in->scalar_type() || grad_in.size(1) != rows_in->size(1)) refuse("the gradient must be like the output of unsort_tokens");
+  }
   const Here here(grad_in, rows_in, offsets, row_of, weights_in);
-  const Tensor grad = unit_rows(grad_in), rows = unit_rows(rows_in);
-  const Maybe weights = weights_in ? Maybe(weights_in->contiguous()) : Maybe();
-  const int64_t t = row_of.size(0), k = row_of.size(1), h = rows.size(1);
+  const Tensor grad = unit_rows(grad_in);
+  const Maybe rows = rows_in ? Maybe(unit_rows(*rows_in)) : Maybe(), weights = weights_in ? Maybe(weights_in->contiguous()) : Maybe();
+  const int64_t t = row_of.size(0), k = row_of.size(1), h = grad.size(1);
   Maybe grad_rows, grad_weights;
-  if (want_rows) grad_rows = fresh({t * k, h}, rows.scalar_type(), rows);
-  if (want_weights && weights) grad_weights = fresh({t, k}, at::kFloat, rows);
-  check(b200moe_unsort_rows_backward(ptr(grad), row_stride(grad), ptr(rows), row_stride(rows), ptr<int32_t>(row_of), ptr<float>(weights), t, (int32_t)k, h,
-                                     row_type(rows.scalar_type()), valid_rows(offsets), ptr(grad_rows), ptr<float>(grad_weights), here.stream()),
+  if (want_rows) grad_rows = fresh({t * k, h}, grad.scalar_type(), grad);
+  if (rows) grad_weights = fresh({t, k}, at::kFloat, grad);
+  check(b200moe_unsort_rows_backward(ptr(grad), row_stride(grad), ptr(rows), row_stride(rows), ptr<int32_t>(row_of), ptr<float>(weights), t, (int32_t)k, h, type,
+                                     valid_rows(offsets), ptr(grad_rows), ptr<float>(grad_weights), here.stream()),
         "b200moe_unsort_rows_backward");
   return {grad_rows, grad_weights};
 }
@@ -315,16 +320,18 @@ struct SortTokens : torch::autograd::Function<SortTokens> {
   }
 };
 
+// What is saved is what a gradient that is asked for reads: the rows, the largest tensor here, only where the weights have one.
 struct UnsortTokens : torch::autograd::Function<UnsortTokens> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Maybe& weights, const Tensor& offsets, const Tensor& row_of) {
-    ctx->save_for_backward({rows, weights ? *weights : Tensor(), offsets, row_of});
+    ctx->save_for_backward({weights && weights->requires_grad() ? rows : Tensor(), weights && rows.requires_grad() ? *weights : Tensor(), offsets, row_of});
     return unsort_rows(rows, offsets, row_of, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const bool weighted = saved[1].defined();
-    auto [grad_rows, grad_weights] = unsort_rows_backward(grads[0].detach(), saved[0].detach(), saved[2], saved[3], weighted ? Maybe(saved[1].detach()) : Maybe(),
-                                                          ctx->needs_input_grad(0), weighted && ctx->needs_input_grad(1));
+    const auto given = [](const Tensor& t) { return t.defined() ? Maybe(t.detach()) : Maybe(); };
+    const bool want_weights = saved[0].defined() && ctx->needs_input_grad(1);
+    auto [grad_rows, grad_weights] = unsort_rows_backward(grads[0].detach(), want_weights ? given(saved[0]) : Maybe(), saved[2], saved[3], given(saved[1]),
+                                                          ctx->needs_input_grad(0));
     return once({grad_rows ? *grad_rows : Tensor(), grad_weights ? *grad_weights : Tensor(), Tensor(), Tensor()});
   }
 };

@@ -344,3 +344,42 @@ def test_function_transforms_and_tangents_raise():
         for i in range(len(args)):
             with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
                 f(*(forward_ad.make_dual(v, o) if j == i else v for j, (v, o) in enumerate(zip(args, ones))))
+
+
+def test_unsort_keeps_only_what_its_gradient_reads():
+    """The rows are read for the weights' gradient, the weights for the rows': what is not read may change before the backward pass, and goes with its
+    last reference."""
+    t, k, e, h = 64, 4, 8, 1024
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    leaf, w, dy = rand((t * k, h), torch.bfloat16, 1).requires_grad_(), rand((t, k), torch.float32, 2), rand((t, h), torch.bfloat16, 3)
+    wl = w.clone().requires_grad_()
+    want_rows, want_w = torch.autograd.grad(ks.unsort_tokens(leaf, order, wl), (leaf, wl), dy)
+    plain, = torch.autograd.grad(ks.unsort_tokens(leaf, order), leaf, dy)
+    for weights, want in ((w, want_rows), (None, plain)):
+        rows = leaf * 1
+        y = ks.unsort_tokens(rows, order, weights)
+        rows.mul_(2)                                               # not read: no error, and the derivative of `rows` as it was
+        got, = torch.autograd.grad(y, leaf, dy)
+        assert torch.equal(got, want)
+        rows = leaf * 1
+        y = ks.unsort_tokens(rows, order, weights)
+        held = torch.cuda.memory_allocated()
+        del rows
+        assert held - torch.cuda.memory_allocated() >= t * k * h * 2
+        assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want)
+    # the weights' gradient alone: the rows are read, the weights are not
+    weights = wl * 1
+    y = ks.unsort_tokens(leaf.detach(), order, weights)
+    weights.mul_(2)
+    assert torch.equal(torch.autograd.grad(y, wl, dy)[0], want_w)
+    rows = leaf.detach().clone()
+    y = ks.unsort_tokens(rows, order, wl)
+    rows.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, wl, dy)
+    # odd widths as well, where a row's phase is worked out from its address
+    for h in (7, 33, 1025):
+        odd, dy = rand((t * k, h), torch.float16, 4).requires_grad_(), rand((t, h), torch.float16, 5)
+        both = torch.autograd.grad(ks.unsort_tokens(odd, order, wl), (odd, wl), dy)
+        assert torch.equal(torch.autograd.grad(ks.unsort_tokens(odd, order, w), odd, dy)[0], both[0])
+        assert torch.equal(torch.autograd.grad(ks.unsort_tokens(odd.detach(), order, wl), wl, dy)[0], both[1])
