@@ -5,7 +5,6 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -276,26 +275,34 @@ std::tuple<Maybe, Maybe> unsort_rows_backward(const Tensor& grad_in, const Maybe
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-bool is_captured(const c10::Stream& stream) {
-  const cudaStream_t handle = c10::cuda::CUDAStream(stream).stream();
+bool is_default(cudaStream_t stream) { return !stream || stream == cudaStreamLegacy; }
+// The capture that a stream takes part in: 0 none (the default stream never does).
+unsigned long long capture_of(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  return handle && cudaStreamIsCapturing(handle, &status) == cudaSuccess && status == cudaStreamCaptureStatusActive;
+  unsigned long long id = 0;
+  return !is_default(stream) && cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess && status == cudaStreamCaptureStatusActive ? id : 0;
 }
 
-// A graph that was built outside a capture and is still alive keeps the gradient node of its leaf on the stream it was built on; a backward pass
-// that is captured would have to wait for that stream, which ends the process inside autograd's worker thread. So the call is refused while
-// it can be: where a node that t's gradient will reach, its leaves' among them, is on a stream that is not captured.
+// A graph that was built outside a capture and is still alive keeps the gradient node of its leaf on the stream it was built on, and a backward pass
+// runs it there. A stream of its own joins the capture through the events that autograd records; the default stream cannot, nor can one that
+// another capture has, and the attempt ends the process inside autograd's worker thread. So the call is refused while it can be: where a
+// node that t's gradient will reach, its leaves' among them, is on such a stream.
 void check_capture(const Tensor& t) {
-  if (!t.is_cuda() || !t.requires_grad() || c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  if (!t.is_cuda() || !t.requires_grad()) return;
+  const unsigned long long capture = capture_of(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+  if (!capture) return;
   std::vector<std::shared_ptr<torch::autograd::Node>> open{t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn()};
   std::unordered_set<torch::autograd::Node*> seen;
   while (!open.empty()) {
     const auto node = open.back();
     open.pop_back();
     if (!node || !seen.insert(node.get()).second) continue;
-    const auto stream = node->stream();
-    if (stream && *stream != c10::cuda::getCurrentCUDAStream(stream->device_index()).unwrap() && !is_captured(*stream))
-      refuse("a graph of this leaf from outside the capture is still alive: let it go, or capture with x.detach().requires_grad_()");
+    if (const auto stream = node->stream()) {
+      const cudaStream_t handle = c10::cuda::CUDAStream(*stream).stream();
+      const unsigned long long other = capture_of(handle);
+      if (is_default(handle) || (other && other != capture))
+        refuse("a graph of this leaf from outside the capture is still alive: let it go, or capture with x.detach().requires_grad_()");
+    }
     for (const auto& edge : node->next_edges()) open.push_back(edge.function);
   }
 }

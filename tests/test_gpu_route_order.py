@@ -383,3 +383,36 @@ def test_unsort_keeps_only_what_its_gradient_reads():
         both = torch.autograd.grad(ks.unsort_tokens(odd, order, wl), (odd, wl), dy)
         assert torch.equal(torch.autograd.grad(ks.unsort_tokens(odd, order, w), odd, dy)[0], both[0])
         assert torch.equal(torch.autograd.grad(ks.unsort_tokens(odd.detach(), order, wl), wl, dy)[0], both[1])
+
+
+def test_capture_beside_a_live_graph_of_a_side_stream():
+    """A stream other than the default one joins a capture when the backward pass reaches its nodes: a leaf whose live graph was built there is taken."""
+    t, k, e, h = 20, 2, 4, 64
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w = rand((t, h), torch.float32, 1).requires_grad_(), rand((t, k), torch.float32, 2).requires_grad_()
+    g, dy = rand((t * k, h), torch.float32, 3), rand((t, h), torch.float32, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive, other = x * 2, w * 2
+    torch.cuda.synchronize()
+
+    def grads(inputs):
+        v, u = inputs()
+        return (torch.autograd.grad((ks.sort_tokens(v, order) * g).sum(), x, retain_graph=True)[0],
+                torch.autograd.grad(ks.unsort_tokens(g, order, u), w, dy, retain_graph=True)[0])
+
+    for inputs in (lambda: (x, w), lambda: (x + 1, w * w), lambda: (alive, other)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = grads(inputs)
+        graph.replay()
+        for got, want in zip(captured, grads(inputs)):
+            assert torch.equal(got, want)
+    # .backward() into .grad
+    x.grad = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (ks.sort_tokens(x, order) * g).sum().backward()
+    graph.replay()
+    assert torch.equal(x.grad, torch.autograd.grad((ks.sort_tokens(x, order) * g).sum(), x)[0])
