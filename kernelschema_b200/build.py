@@ -14,6 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200moe.so")
 SHIM = os.path.join(HERE, "_b200moe_shim.so")
 TORCH_CALLS = os.path.join(HERE, "_b200moe_torch.so")
+TORCH_STAMP = os.path.join(HERE, "build", "torch_calls.torch")      # the torch and Python that TORCH_CALLS was built for
 SOURCES = ["quantize.cu", "router.cu", "route_map.cu", "gather.cu", "finalize.cu", "gemm_nvfp4.cu", "gemm_w4a16.cu", "gemm_w4a16_decode.cu", "gemm_w4a16_expand.cu", "ep_exchange.cu", "rowquant.cu", "gemm_8bit.cu", "gemm_8bit_decode.cu", "route_order.cu", "api.cu"]
 HEADERS = ["gemm_8bit.cuh", "gemm_8bit_clusters.cuh", "kernels.cuh", "ptx.cuh", "quantize.cuh", "rows.cuh", "topk.cuh", "w4a16.cuh", os.path.join("..", "..", "include", "b200moe.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -82,11 +83,17 @@ def build_shim(force: bool = False) -> str:
 
 
 def build_torch_calls(force: bool = False) -> str:
-    """Compile the calls on torch tensors (C++ against torch's headers; links the in-tree libb200moe.so through $ORIGIN)."""
+    """Compile the calls on torch tensors (C++ against torch's headers; links the in-tree libb200moe.so through $ORIGIN), again where torch or
+    Python is another than it was built for."""
+    import torch
     src = os.path.join(CSRC, "torch_calls.cpp")
-    if force or _stale(TORCH_CALLS, [src, LIB, os.path.join(CSRC, "..", "..", "include", "b200moe.h")]):
+    wanted = f"torch {torch.__version__} python {sys.version_info[0]}.{sys.version_info[1]}\n"
+    built_for = None
+    if os.path.exists(TORCH_STAMP):
+        with open(TORCH_STAMP) as f:
+            built_for = f.read()
+    if force or built_for != wanted or _stale(TORCH_CALLS, [src, LIB, os.path.join(CSRC, "..", "..", "include", "b200moe.h")]):
         import sysconfig
-        import torch
         base = os.path.dirname(torch.__file__)
         cuda = os.path.dirname(os.path.dirname(_nvcc()))
         cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
@@ -96,6 +103,9 @@ def build_torch_calls(force: bool = False) -> str:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError("build of the torch calls failed:\n" + res.stderr)
+        os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
+        with open(TORCH_STAMP, "w") as f:
+            f.write(wanted)
     return TORCH_CALLS
 
 

@@ -127,3 +127,30 @@ def test_w4a16_scratch_of_a_captured_call_lies_in_a_graph_pool(monkeypatch):
     monkeypatch.setattr(torch, "empty", no_memory)
     for capturing in (False, True):
         assert ops._w4a16_expanded(dev, 4096) is None
+
+
+def test_torch_calls_are_built_again_for_another_torch(tmp_path, monkeypatch):
+    """File times say nothing of the torch that the extension was compiled against: a change of its version, or an unknown one, builds it again."""
+    import types
+    import torch
+    from kernelschema_b200 import build
+    build.build()
+    runs = []
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **_: runs.append(cmd) or types.SimpleNamespace(returncode=0, stderr=""))
+    monkeypatch.setattr(build, "TORCH_STAMP", str(tmp_path / "stamps" / "torch"))
+    build.build_torch_calls()                                # built for an unknown torch
+    build.build_torch_calls()
+    assert len(runs) == 1 and build.TORCH_CALLS in runs[0]
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    build.build_torch_calls()
+    build.build_torch_calls()
+    assert len(runs) == 2
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **_: types.SimpleNamespace(returncode=1, stderr="no"))
+    monkeypatch.setattr(torch, "__version__", "0.1")
+    for _ in range(2):                                       # a build that failed is not taken for one
+        try:
+            build.build_torch_calls()
+        except RuntimeError as exc:
+            assert "no" in str(exc)
+        else:
+            raise AssertionError("not built again")
