@@ -16,7 +16,7 @@ SHIM = os.path.join(HERE, "_b200moe_shim.so")
 TORCH_CALLS = os.path.join(HERE, "_b200moe_torch.so")
 TORCH_STAMP = os.path.join(HERE, "build", "torch_calls.torch")      # the torch and Python that TORCH_CALLS was built for
 SOURCES = ["quantize.cu", "router.cu", "route_map.cu", "gather.cu", "finalize.cu", "gemm_nvfp4.cu", "gemm_w4a16.cu", "gemm_w4a16_decode.cu", "gemm_w4a16_expand.cu", "ep_exchange.cu", "rowquant.cu", "gemm_8bit.cu", "gemm_8bit_decode.cu", "route_order.cu", "api.cu"]
-HEADERS = ["gemm_8bit.cuh", "gemm_8bit_clusters.cuh", "kernels.cuh", "ptx.cuh", "quantize.cuh", "rows.cuh", "topk.cuh", "w4a16.cuh", os.path.join("..", "..", "include", "b200moe.h")]
+HEADERS = ["gemm_8bit.cuh", "gemm_8bit_clusters.cuh", "gemm_8bit_plan.cuh", "kernels.cuh", "ptx.cuh", "quantize.cuh", "rows.cuh", "topk.cuh", "w4a16.cuh", os.path.join("..", "..", "include", "b200moe.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Xptxas", "-v"]
 

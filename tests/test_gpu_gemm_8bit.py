@@ -199,3 +199,52 @@ def test_empty_captured_and_repeated():
     torch.cuda.synchronize()
     for o in outs[0] + outs[1]:
         assert torch.equal(o, got[0])
+
+
+# the forms that the shapes above leave out for one type of codes or for both (which form a call takes: test_host_rules.py)
+MORE_SHAPES = [(1, 4861, 5312), (3, 5425, 3376), (1, 2401, 12800), (5, 2959, 6960), (9, 1001, 24592), (16, 513, 32784), (17, 5513, 3568), (19, 4175, 2880), (391, 591, 4528),
+               (683, 123, 1744), (677, 125, 3344)]
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("m,n,k", MORE_SHAPES)
+def test_dense_of_the_other_forms(m, n, k, kind):
+    test_dense(m, n, k, kind)
+
+
+# (counts, rows behind, first row): on CTA pairs above 160 rows a segment, K >= 1536 and N > 128; single tiles of 64 and 128 that are more than the device runs at once
+MORE_GROUPS = [([100, 700, 0, 257, 1, 513, 333, 161], 57, 3, 200, 1536), ([100, 700, 0, 257, 1, 513, 333, 161], 0, 0, 384, 2064), ([300, 150] * 10, 9, 65, 129, 1552),
+               ([1500], 1, 2, 2049, 1536), ([0, 1025, 0, 32, 511, 224], 300, 1, 1000, 1600), ([20] * 30, 2, 1, 1000, 272), ([40] * 30, 5, 7, 1000, 272), ([200, 0, 64, 33] * 8, 3, 0, 384, 2064)]
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("case", range(len(MORE_GROUPS)))
+def test_grouped_of_the_other_forms(case, kind):
+    """Uneven segments that start anywhere, tiles of 32 to 256 rows, weight rows of the next expert in a tile, rows in front of and behind the segments."""
+    counts, behind, lead, n, k = MORE_GROUPS[case]
+    e, m, end = len(counts), lead + sum(counts) + behind, lead + sum(counts)
+    off = segments(counts, lead)
+    a, b, sa, sb = codes((m, k), kind, 1), codes((e, n, k), kind, 2), scales(m, 3), scales(e * n, 4).view(e, n)
+    at = off.tolist()
+    for out_dtype in (torch.bfloat16, torch.float32):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = ks.mm_8bit_grouped(a, sa, b, sb, off, out_dtype=out_dtype, status=status)
+        given = torch.full((m, n + 3), -17.0, dtype=out_dtype, device="cuda")
+        ks.mm_8bit_grouped(a, sa, b, sb, off, out=given[:, 1:-2], status=status)
+        assert int(status) == 0
+        assert torch.equal(given[lead:end, 1:-2], out[lead:end]) and not bool(out[:lead].any()) and not bool(out[end:].any())
+        assert bool((given[:lead] == -17).all()) and bool((given[end:] == -17).all()) and bool((given[:, 0] == -17).all()) and bool((given[:, -2:] == -17).all())
+        for i in range(e):
+            if counts[i]:
+                check(out[at[i]:at[i + 1]], a[at[i]:at[i + 1]], sa[at[i]:at[i + 1]], b[i], sb[i])
+
+
+@pytest.mark.parametrize("kind", CODES)
+@pytest.mark.parametrize("m,n,k", ((1, 200, 512), (5, 192, 512), (64, 192, 512), (700, 512, 192), (700, 384, 1536)))
+def test_dense_and_grouped_agree(m, n, k, kind):
+    """One segment of all rows is the dense product: the same bits in int8, sums in another order in e4m3."""
+    a, b, sa, sb = codes((m, k), kind, 1), codes((n, k), kind, 2), scales(m, 3), scales(n, 4)
+    dense, grouped = ks.mm_8bit(a, sa, b, sb), ks.mm_8bit_grouped(a, sa, b[None], sb[None], segments([m]))
+    check(dense, a, sa, b, sb)
+    check(grouped, a, sa, b, sb)
+    assert kind == "e4m3" or torch.equal(dense, grouped)

@@ -154,3 +154,48 @@ def test_torch_calls_are_built_again_for_another_torch(tmp_path, monkeypatch):
             assert "no" in str(exc)
         else:
             raise AssertionError("not built again")
+
+
+def test_forms_of_the_8bit_products(tmp_path):
+    """The shapes of the GPU tests reach every form that a call of any size takes, in both types of codes; the rule for experts' segments changes where it says."""
+    import random
+    from kernelschema_b200 import build
+    from test_gpu_gemm_8bit import GROUPS, MORE_GROUPS, MORE_SHAPES, SHAPES
+    src, exe = tmp_path / "forms.cu", str(tmp_path / "forms")
+    src.write_text("""#include <stdio.h>
+#include "gemm_8bit_plan.cuh"
+using namespace b200;
+int main() {
+  long long m, n, k, experts, code;
+  while (scanf("%lld %lld %lld %lld %lld", &m, &n, &k, &experts, &code) == 5) {
+    Gemm8Params p{};
+    p.M = (int)m, p.N = (int)n, p.K = (int)k, p.experts = (int)experts, p.code = (int)code;
+    const G8Plan plan = experts ? grouped_plan(p) : dense_plan(p, 148);
+    const char* form[] = {"decode", "single", "split", "pair"};
+    printf("%s %d %d %s\\n", form[plan.form], plan.mt, plan.split, plan.form != kDecode && g8_deep(plan, g8_items(p, plan), 148) ? "deep" : "shared");
+  }
+}""")
+    subprocess.run([build._nvcc(), "-std=c++17", "-I", os.path.join(ROOT, "kernelschema_b200", "csrc"), str(src), "-o", exe], check=True)
+
+    def forms(calls):
+        text = "\n".join(" ".join(map(str, c)) for c in calls)
+        return subprocess.run([exe], input=text, check=True, capture_output=True, text=True).stdout.splitlines()
+
+    dense = {"decode 0 1 shared", "pair 128 1 shared", "pair 256 1 shared", "split 16 4 shared", "split 16 8 shared", "split 16 8 deep", "split 64 4 shared",
+             "split 64 8 shared", "split 64 8 deep", "split 128 8 shared", "split 128 8 deep"} | {f"single {mt} 1 {s}" for mt in (16, 64, 128) for s in ("deep", "shared")}
+    grouped = {f"single {mt} 1 {s}" for mt in (16, 64, 128) for s in ("deep", "shared")} | {"pair 256 1 shared"}
+    rng = random.Random(1)
+    log = lambda lo, hi: int(lo * (hi / lo) ** rng.random())  # noqa: E731
+    for code in (0, 1):
+        assert set(forms([(m, n, k, 0, code) for m, n, k in SHAPES + MORE_SHAPES])) == dense
+        assert set(forms([(log(1, 20000), log(1, 40000), 16 * log(1, 8000), 0, code) for _ in range(100000)])) == dense
+        groups = [(sum(c) + behind, n, k, len(c), code) for c, behind in GROUPS for n, k in ((128, 128), (200, 272), (33, 1040))]
+        groups += [(lead + sum(c) + behind, n, k, len(c), code) for c, behind, lead, n, k in MORE_GROUPS]
+        assert set(forms(groups)) == grouped
+        assert set(forms([(log(1, 100000), log(1, 20000), 16 * log(1, 1000), log(1, 1024), code) for _ in range(100000)])) == grouped
+    # both ways of the decode kernel: 16 tokens, 32 in int8
+    assert forms([(17, 256, 512, 0, 0), (17, 256, 512, 0, 1), (16, 256, 512, 0, 1)])[0::2] == ["decode 0 1 shared"] * 2
+    edges = [(4, "single 16"), (5, "single 64"), (32, "single 64"), (33, "single 128"), (160, "single 128"), (161, "pair 256")]
+    for rows, want in edges:
+        assert forms([(rows * 8, 256, 1536, 8, 0)])[0].startswith(want)
+    assert forms([(2000, 256, 1520, 8, 0), (2000, 128, 1536, 8, 0), (2000, 129, 1536, 8, 0)]) == ["single 128 1 deep"] * 2 + ["pair 256 1 shared"]
