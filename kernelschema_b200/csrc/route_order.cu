@@ -38,7 +38,7 @@ struct OrderView {
 
 DEV int bucket_of(const OrderView& v, int64_t f) {
   if (f >= v.total) return -1;
-  const int64_t t = v.total <= INT32_MAX ? (int64_t)((uint32_t)f / (uint32_t)v.K) : f / v.K;
+  const int64_t t = (uint32_t)f / (uint32_t)v.K;             // fewer than 2^31 routes
   const int e = __ldg(v.ids + t * v.stride + (f - t * v.K));
   return (uint32_t)e < (uint32_t)v.E ? e : v.E;
 }

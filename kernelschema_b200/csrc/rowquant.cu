@@ -468,7 +468,9 @@ int launch_rows(const typename K::P& p, cudaStream_t st) {
   while (threads() > (values <= 16 ? 1024 : 512)) values *= 2;
   if (values == 8) return launch_form<K, 8 / E, false, kAny>(p, threads(), 32, st);
   if (values == 16) return launch_form<K, 16 / E, false, kAny>(p, threads(), 32, st);
-  if (values == 32) return launch_form<K, 32 / E, false, kAny>(p, threads(), 32, st);
+  if constexpr (!kAny && K::kValues == 32) {                 // elsewhere the step from 16 values leads past 32: as many columns fit 16
+    if (values == 32) return launch_form<K, 32 / E, false, kAny>(p, threads(), 32, st);
+  }
   return launch_form<K, 64 / E, false, kAny>(p, threads(), 32, st);
 }
 
