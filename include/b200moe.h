@@ -180,18 +180,20 @@ int b200moe_gemm_bf16_nvfp4(const void* a, int64_t a_stride, const void* b_q, co
  * residual may be NULL (h = x); hidden (h) and normed (y), in the rows' type `dtype`, are written where not NULL. hidden may be x or
  * residual itself. weight: [cols] in the rows' type or fp32. Strides in elements between rows (0 repeats one input row). Sums in fp32; h is not
  * rounded before the norm. A row whose max|y| is below 2^-116 has scale 0 and codes 0; a row with a NaN or an infinity in it, or
- * with a sum of squares beyond fp32, has scale NaN and codes 0. Any width and alignment; 16-byte aligned rows are the fast ones. */
+ * with a sum of squares beyond fp32, has scale NaN and codes 0; so has, with eps = 0, a row of zeros or one
+ * whose squares vanish in fp32 (0 * infinity). Any width and alignment; 16-byte aligned rows are the fast ones. */
 int b200moe_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
                              int32_t weight_dtype, int64_t rows, int64_t cols, float eps, int32_t dtype, int32_t q_type, void* q,
                              int64_t q_stride, float* scale, void* hidden, int64_t hidden_stride, void* normed, int64_t normed_stride,
                              void* stream);
-/* SwiGLU with a quantised output: x = [gate | up] of 2 * cols columns, y = gate * sigmoid(gate) * up, scale and q as above. */
+/* SwiGLU with a quantised output: x = [gate | up] of 2 * cols columns, y = gate * sigmoid(gate) * up, scale and q as above (a
+ * row with a y beyond fp32 has scale NaN as well). */
 int b200moe_swiglu_quantize(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int32_t dtype, int32_t q_type, void* q,
                             int64_t q_stride, float* scale, void* stream);
 
 /* GEMM of 8-bit rows: out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] * b[n, k]. a [M, K] and b [N, K] both int8 (sums exact in int32) or both
- * E4M3 (sums in fp32), K % 16 == 0 and K <= 131071, 16-byte aligned, a_stride (bytes between rows of a) a multiple of 16; scales fp32; out
- * [M, N] bf16, fp16 or fp32, any N and out_stride. status as in b200moe_gemm_nvfp4. */
+ * E4M3 (sums in fp32), K % 16 == 0 and K <= 131071, 16-byte aligned, a_stride (bytes between rows of a) a multiple of 16; scales fp32 (the
+ * sum is multiplied by a_scale, then by b_scale, in fp32); out [M, N] bf16, fp16 or fp32, any N and out_stride. status as in b200moe_gemm_nvfp4. */
 int b200moe_gemm_8bit(const void* a, int64_t a_stride, const float* a_scale, const void* b, const float* b_scale, void* out, int64_t m,
                       int64_t n, int64_t k, int64_t out_stride, int32_t code, int32_t out_type, int32_t* status, void* stream);
 /* The same over segments of rows, each with its own weights: rows offsets[e] .. offsets[e + 1] - 1 (device int32 [experts + 1], ascending) times

@@ -8,8 +8,8 @@
 // kind::i8 and kind::f8f6f4 take 32 bytes of K per instruction, four per step of 128 bytes. K beyond the last step reads as zeros (TMA's fill), so
 // rows need no more than 16-byte lengths.
 //
-// What bounds it: many tokens, the tensor cores (8192 x 4096 x 12288 int8 256 us = 3.2 P op/s, 96 % busy; sustained, the power cap); few, the weight
-// stream (64 tokens over 128 experts 305 MB in 53 us = 5.9 TB/s) and, below about 20 MB of weights, launch, first access and
+// What bounds it: many tokens, the tensor cores (8192 x 4096 x 12288 int8 256 us in a graph = 3.2 P op/s, 96 % busy; in calls among others 297, by the power cap); few, the weight
+// stream (64 tokens over 128 experts 305 MB in 53 us = 5.75 TB/s) and, below about 20 MB of weights, launch, first access and
 // reduction (100 x 2113 x 7168 10.7 us). The forms and their times are at dense_plan (gemm_8bit_plan.cuh).
 #include "gemm_8bit.cuh"
 #include "gemm_8bit_clusters.cuh"

@@ -79,7 +79,8 @@ inline G8Plan dense_plan(const Gemm8Params& p, int sms) {
   return best;
 }
 
-// Grouped: by the rows of a segment, on average, which is all that the host knows. Weights stream past few rows whatever the tile; from 32 rows on a
+// Grouped: by the rows of a segment, on average, which is all that the host knows (few segments that hold all rows take tiles as small as the average of all
+// segments asks for, and their weights then come from L2 once per tile). Weights stream past few rows whatever the tile; from 32 rows on a
 // tile should hold a segment, and from about 160 the pair's tile saves operand traffic, unless K is over before its longer start is made
 // up for (us, 128 experts: 1536 x 2048 with 2 rows 43 / 45 / 46 / 46 for 16 / 64 / 128 / pairs, 32 rows 77 / 70 / 70 / 70, 256 rows - / 166 / 140 / 128,
 // 1024 rows - / - / 415 / 323; 2048 x 768 with 512 rows 141 for 128, 162 for pairs).

@@ -4,11 +4,12 @@
 //   both       amax = max|y|,  scale = amax / Q,  q = round_to_nearest_even(y * (Q / amax)),  Q = 127 (int8) or 448 (e4m3)
 //
 // Both are bound by HBM: every input element is read once, every output element written once, and a row stays in registers between its
-// reductions (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 43 us = 5.8, 16384 x 2048 27 = 6.2). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
+// reductions, but for a part of the widest ones, which spills (shifted rows above 16384 columns, fp32 above 8192; aligned fp32 above 16384) (norm 8192 x 7168 bf16 68 us = 6.1 TB/s; SwiGLU 65536 x 768 43 us = 5.8, 16384 x 2048 27 = 6.2). h, the sum of squares, y and amax are fp32; the residual stream h, the normed row y and the code q are each rounded once,
 // from the fp32 value (the norm sees h before it is rounded to the stream's type).
 // A row holds no scale when it has no finite amax: a NaN or an infinity in it, or a sum of squares beyond fp32, makes the scale NaN and
 // the codes zero, so that the row is NaN wherever it is multiplied out. A row whose amax is below 2^-116 counts as zero (scale 0,
-// codes 0): Q / amax stays finite for every other one, and scale stays a normal number.
+// codes 0): Q / amax stays finite for every other one, and scale stays a normal number. Without eps the norm of a row of zeros, or of one whose squares
+// vanish in fp32, is 0 * infinity: scale NaN. A y on the border between two codes may take either: y * (Q / amax) and y / scale round differently.
 //
 // Rows that vectors do not fit (odd widths, strides or addresses) are read as vectors shifted into place (Any16), so a thread holds the
 // same columns as otherwise, and written through shared memory, from where they go out in aligned vectors with single elements at the two ends.
@@ -432,7 +433,7 @@ struct SwigluKernels {
   using P = SwigluParams;
   using I = T;
   static constexpr int kStageSize = 1;
-  static constexpr int kValues = 16, kValuesAny = sizeof(T) == 2 ? 16 : 8;         // 16384 x 2048 bf16 27.7 us with 16, 29.4 with 32
+  static constexpr int kValues = 16, kValuesAny = sizeof(T) == 2 ? 16 : 8;         // 16384 x 2048 bf16 27.2 us with 16, 27.7 with 32
   template <int VPT, bool kWarp, bool kAny>
   static constexpr auto kernel() { return k_swiglu_quantize<T, VPT, kWarp, kAny>; }
 };

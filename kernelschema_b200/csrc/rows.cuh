@@ -90,7 +90,7 @@ struct Any16 {
   }
 };
 // The same interface for addresses that are aligned. kZero: a vector that is not wanted is zero, which makes the load a predicated one among the
-// others (unsort 8192 x 8 x 2048 50 us, 71 without); a warp's row is better without (SwiGLU 65536 x 768 45 us, 48 with), and its kernel looks at
+// others (unsort 8192 x 8 x 2048 50 us, 71 without); a warp's row is better without (SwiGLU 65536 x 768 43.4 us, 43.8 with), and its kernel looks at
 // no vector that was not wanted.
 template <class T, bool kZero>
 struct Own16 {

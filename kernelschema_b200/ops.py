@@ -249,14 +249,14 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     fp32. ``hidden`` is h in x's type (x itself without a residual); ``normed`` is y in x's type where asked for, else None. ``out`` = (q,
     scale, hidden, normed): caller-owned buffers, each may be None; hidden may be x or residual themselves (in place).
     h and the sums are fp32, and h is not rounded before the norm. A row of zeros (max|y| < 2^-116) has scale 0; a row with a NaN or an infinity, or whose
-    squares' sum leaves fp32, has scale NaN and codes 0. For inference: this and the other 8-bit operators have no gradient, `hidden` included,
+    squares' sum leaves fp32, has scale NaN and codes 0, and with eps = 0 a row of zeros or of squares that vanish in fp32 too (0 * infinity). For inference: this and the other 8-bit operators have no gradient, `hidden` included,
     and refuse tensors that require one while grad mode is on (parameters: call under `torch.no_grad()`)."""
     return _calls().rmsnorm_quantize(x, weight, residual, eps, dtype, normed, *(out or (None, None, None, None)))
 
 
 def swiglu_quantize(x: torch.Tensor, dtype: torch.dtype = torch.int8, out=None):
     """x = [gate | up] (bf16, fp16 or fp32 [T, 2I], I <= 32768) -> (q [T, I], scale fp32 [T]) of gate * sigmoid(gate) * up: the step between the two 8-bit
-    products of a feed-forward layer or an expert. dtype, scales, special rows and ``out`` = (q, scale) as in `rmsnorm_quantize`."""
+    products of a feed-forward layer or an expert (gate first; the NVFP4 layer's weight rows are up, then gate, before they are prepared). dtype, scales, special rows and ``out`` = (q, scale) as in `rmsnorm_quantize`."""
     return _calls().swiglu_quantize(x, dtype, *(out or (None, None)))
 
 
