@@ -314,12 +314,17 @@ variable_list once(variable_list grads) {
       .apply(std::move(grads));
 }
 
+void refuse_tangents(bool any) {
+  if (any) refuse("sort_tokens and unsort_tokens have no forward-mode derivative");
+}
+
 struct SortTokens : torch::autograd::Function<SortTokens> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets, const Tensor& row_of) {
     ctx->save_for_backward({offsets, row_of});
     return sort_rows(x, offsets, row_of);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(has_tangent(grads[0]));                  // forward mode over this pass: the inputs need not carry any
     const variable_list saved = ctx->get_saved_variables();
     const Tensor grad = grads[0].detach();
     const Tensor dx = grad.dim() == 1 ? unsort_rows(grad.unsqueeze(1), saved[0], saved[1], {}).squeeze(1) : unsort_rows(grad, saved[0], saved[1], {});
@@ -334,6 +339,7 @@ struct UnsortTokens : torch::autograd::Function<UnsortTokens> {
     return unsort_rows(rows, offsets, row_of, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(has_tangent(grads[0]));
     const variable_list saved = ctx->get_saved_variables();
     const auto given = [](const Tensor& t) { return t.defined() ? Maybe(t.detach()) : Maybe(); };
     const bool want_weights = saved[0].defined() && ctx->needs_input_grad(1);
@@ -342,10 +348,6 @@ struct UnsortTokens : torch::autograd::Function<UnsortTokens> {
     return once({grad_rows ? *grad_rows : Tensor(), grad_weights ? *grad_weights : Tensor(), Tensor(), Tensor()});
   }
 };
-
-void refuse_tangents(bool any) {
-  if (any) refuse("sort_tokens and unsort_tokens have no forward-mode derivative");
-}
 
 Tensor sort_tokens(const Tensor& x, const Tensor& offsets, const Tensor& row_of) {
   refuse_tangents(has_tangent(x));

@@ -6,8 +6,8 @@
 
 `mm_8bit_grouped` takes the sorted rows and the offsets. Every computation runs in libb200moe.so. In a CUDA graph the gradients are captured like the
 rest; a call whose leaf still has a live graph that was built on the default stream is refused (capture with ``x.detach().requires_grad_()``). The derivatives
-are those of reverse mode, once: an input with a tangent of forward mode (`torch.autograd.forward_ad`) is refused, and `torch.func`
-transforms raise."""
+are those of reverse mode, once: an input, or an incoming gradient, with a tangent of forward mode (`torch.autograd.forward_ad`) is refused, and
+`torch.func` transforms raise."""
 from __future__ import annotations
 
 from typing import NamedTuple

@@ -416,3 +416,18 @@ def test_capture_beside_a_live_graph_of_a_side_stream():
         (ks.sort_tokens(x, order) * g).sum().backward()
     graph.replay()
     assert torch.equal(x.grad, torch.autograd.grad((ks.sort_tokens(x, order) * g).sum(), x)[0])
+
+
+def test_a_gradient_with_a_tangent_is_refused():
+    """Forward mode over a backward pass: the gradient that comes in carries a tangent though no input does."""
+    import torch.autograd.forward_ad as forward_ad
+    t, k, e, h = 12, 2, 4, 32
+    order = ks.route_sort(make_ids(t, k, e, 1), e)
+    x, w, rows = (v.requires_grad_() for v in (rand((t, h), torch.float32, 1), rand((t, k), torch.float32, 2), rand((t * k, h), torch.float32, 3)))
+    for y, leaves in ((ks.sort_tokens(x, order), (x,)), (ks.unsort_tokens(rows, order, w), (rows, w)), (ks.unsort_tokens(rows, order), (rows,))):
+        with forward_ad.dual_level():
+            c = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises((RuntimeError, ValueError), match="forward-mode"):
+                torch.autograd.grad((y * c).sum(), leaves, retain_graph=True)
+        for g in torch.autograd.grad(y.sum(), leaves):             # and the call is one like any other without it
+            assert bool(g.isfinite().all())
