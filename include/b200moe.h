@@ -221,7 +221,8 @@ int b200moe_sort_rows(const void* x, int64_t x_stride, int64_t num_tokens, int64
 int b200moe_unsort_rows(const void* rows, int64_t rows_stride, int64_t num_rows, const int32_t* row_of, const float* weights, int64_t num_tokens,
                         int32_t top_k, int64_t cols, int32_t dtype, void* out, int64_t out_stride, void* stream);
 /* Gradients of the above: grad_rows[row_of[t, k]] = weights[t, k] * grad_out[t] ([T * top_k, cols] contiguous, zero from *valid_rows on),
- * grad_weights[t, k] = <rows[row_of[t, k]], grad_out[t]> (fp32; 0 where there is no route). Either may be NULL. */
+ * grad_weights[t, k] = <rows[row_of[t, k]], grad_out[t]> (fp32; 0 where there is no route). Either may be NULL; rows are read for grad_weights alone,
+ * and may be NULL without it. */
 int b200moe_unsort_rows_backward(const void* grad_out, int64_t grad_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
                                  const float* weights, int64_t num_tokens, int32_t top_k, int64_t cols, int32_t dtype,
                                  const int32_t* valid_rows, void* grad_rows, float* grad_weights, void* stream);
